@@ -438,6 +438,65 @@ int rag_index_hybrid_mmr_batch_device(rag_index_t* h, int64_t nq, const float* q
                                       double mmr_lambda, double mmr_threshold, int mmr_metric, int max_results,
                                       int64_t* ids_dev, double* scores_dev, int32_t* n_out_dev, void* stream);
 
+/* ---- rows kept at four bits ---------------------------------------------------------------
+ * The reference hands a `quantization_config` to a collection (vector_db/search_optimizer.py:51,130) and its server then
+ * keeps and scans a compressed copy.  Here a row is stored as four-bit values with one power-of-two scale per group of 32
+ * consecutive elements (the MX layout: e2m1 values, e8m0 scales):
+ *     value(i) = sign * T[code] * 2^(scale - 127),   T = 0, 0.5, 1, 1.5, 2, 3, 4, 6;   scale 255: the group is NaN
+ * 0.53 bytes per element: 100M rows of 768 take 42 GB instead of 307.
+ * Quantising a group with largest magnitude a, f = floor(log2 a): scale 2^s with s = f - 2, or f - 1 where a / 2^f > 1.75,
+ * kept within [-126, 125] (a = 0: -126); codes are the nearest table values to |x| / 2^s, ties to the even code, at most 6.
+ * A group that holds a NaN or an infinity is stored as NaN.
+ *
+ * The buffers belong to the caller (rag_mx4_layout gives the bytes of a row); every call is enqueued on `stream` of
+ * st->device and not synchronised, keeps nothing between calls and allocates nothing, so it may be captured into a graph.
+ * Calls that write one store and calls that use it are ordered by the caller's streams. */
+enum rag_mx4_type { RAG_MX4_F32 = 0, RAG_MX4_BF16 = 1, RAG_MX4_F16 = 2 };
+typedef struct rag_mx4_store {
+    void* codes;      /* n * code_bytes, device memory on a 16-byte boundary; the layout inside a row is the library's own */
+    void* scales;     /* n * scale_bytes, likewise; zero bytes behind a row's groups */
+    int64_t n;        /* rows, at most 2^31 - 1 */
+    int32_t dim;      /* 1 .. 8192 */
+    int32_t device;
+} rag_mx4_store_t;
+/* Bytes of one row.  Block b = i / 128 of a row holds element i at half-byte i % 128 of its 64 bytes; the scale of group
+ * G = i / 32 is byte (G / 16) * 16 + (G % 4) * 4 + (G / 4) % 4.  Elements from dim to the end of the last block are zero. */
+int rag_mx4_layout(int dim, int64_t* code_bytes, int64_t* scale_bytes);
+/* Quantise `count` rows of x_dev (elements of x_type, x_stride elements from row to row) as they are written:
+ *   rows_dev NULL   to the rows [first, first + count)
+ *   rows_dev        to the positions it names; a position outside [0, n) is skipped, of several rows for one position the last is
+ *                   kept.  owner_dev: n int32, zero before the first such call; the call leaves them zero.
+ *   normalize       1: every row is divided by its norm first (COSINE; sum of squares in fp64; a zero row stays zero) */
+int rag_mx4_write_device(const rag_mx4_store_t* st, int64_t first, const int64_t* rows_dev, int32_t* owner_dev, int64_t count,
+                         const void* x_dev, int x_type, int64_t x_stride, int normalize, void* stream);
+/* out_dev[count][dim] (out_type, rounded once to nearest even) = the values of the rows at rows_dev; a position outside
+ * [0, n) -- an unfilled slot of a search -- reads as zeros */
+int rag_mx4_read_device(const rag_mx4_store_t* st, const int64_t* rows_dev, int64_t count, void* out_dev, int out_type, void* stream);
+/* out_dev[i * out_stride + r - row_begin] = sum over the elements of q_i * value(row r), r in [row_begin, row_end): the product
+ * itself, in fp32 (normalize 1: of q_i / |q_i|).  A query that holds a NaN or an infinity gets NaN against every row. */
+int rag_mx4_scores_device(const rag_mx4_store_t* st, int64_t row_begin, int64_t row_end, int64_t nq, const void* q_dev, int q_type,
+                          int64_t q_stride, int normalize, float* out_dev, int64_t out_stride, void* stream);
+/* The same for ragged groups: group g multiplies its queries [groups[4g], groups[4g + 1]) with its rows [groups[4g + 2],
+ * groups[4g + 3]) (groups may share queries and rows, and be empty); its scores, [queries][rows], follow those of group g - 1 in out_dev.  rag_mx4_plan_groups
+ * (host memory, no GPU) checks the groups and cuts them into pieces of RAG_MX4_ITEM_BYTES for the kernel:
+ *   items_out   max_items pieces; *n_items says how many there are (more than max_items: call again with room for them)
+ *   out_begin   NULL or, per group, where its scores start;  *total: how many there are;  *widest: for the product call
+ * The pieces, copied to device memory, serve any number of products with queries of this count and type over a store
+ * of at least n rows. */
+#define RAG_MX4_ITEM_BYTES 32
+int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngroups, const int64_t* groups, int64_t max_items,
+                        void* items_out, int64_t* n_items, int64_t* out_begin, int64_t* total, int32_t* widest);
+int rag_mx4_scores_grouped_device(const rag_mx4_store_t* st, int64_t nq, const void* q_dev, int q_type, int64_t q_stride, int normalize,
+                                  const void* items_dev, int64_t n_items, int32_t widest, float* out_dev, void* stream);
+/* rag_index_search_device over such a store: the k best of every query under the scores above, with the library's order rule
+ * and empty slots; I are row positions.  NaN scores are never returned; row_mask_dev and active_dev: NULL or n bytes each, a
+ * row may be returned where neither is 0.  The workspace (device memory on a 256-byte boundary,
+ * at least rag_mx4_search_workspace(n, nq, k) bytes; -1: bad sizes) must not be shared by searches that may overlap. */
+int64_t rag_mx4_search_workspace(int64_t n, int64_t nq, int k);
+int rag_mx4_search_device(const rag_mx4_store_t* st, int64_t nq, const void* q_dev, int q_type, int64_t q_stride, int normalize, int k,
+                          float min_score, const uint8_t* row_mask_dev, const uint8_t* active_dev, float* D_dev, int64_t* I_dev, void* workspace_dev,
+                          int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

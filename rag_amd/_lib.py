@@ -26,6 +26,8 @@ RAG_OK, RAG_ERR_INVALID, RAG_ERR_HIP, RAG_ERR_OOM, RAG_ERR_UNSUPPORTED = 0, 1, 2
 METRIC_IP, METRIC_COSINE, METRIC_L2 = 0, 1, 2
 KIND_FLAT, KIND_IVF = 0, 1
 MMR_COSINE, MMR_DOT, MMR_EUCLIDEAN = 0, 1, 2
+MX4_F32, MX4_BF16, MX4_F16 = 0, 1, 2
+MX4_ITEM_BYTES = 32
 
 _vp, _i32, _i64, _f32, _f64 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double
 
@@ -82,6 +84,15 @@ SIGNATURES = {
                                                   _i32, _i32, _vp, _vp, _vp, _vp]),
     "rag_index_hybrid_mmr_device": (_i32, [_vp, _vp, _i32, _f32, _i32, _vp, _i64, _vp, _vp, _f64, _f64, _i32, _f64, _f64,
                                            _i32, _i32, _vp, _vp]),
+    "rag_mx4_layout": (_i32, [_i32, C.POINTER(_i64), C.POINTER(_i64)]),
+    "rag_mx4_write_device": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _i64, _i32, _vp]),
+    "rag_mx4_read_device": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp]),
+    "rag_mx4_scores_device": (_i32, [_vp, _i64, _i64, _i64, _vp, _i32, _i64, _i32, _vp, _i64, _vp]),
+    "rag_mx4_plan_groups": (_i32, [_i32, _i32, _i64, _i64, _i64, _vp, _i64, _vp, C.POINTER(_i64), _vp, C.POINTER(_i64),
+                                   C.POINTER(_i32)]),
+    "rag_mx4_scores_grouped_device": (_i32, [_vp, _i64, _vp, _i32, _i64, _i32, _vp, _i64, _i32, _vp, _vp]),
+    "rag_mx4_search_workspace": (_i64, [_i64, _i64, _i32]),
+    "rag_mx4_search_device": (_i32, [_vp, _i64, _vp, _i32, _i64, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "rag_multi_create": (_i32, [_i32, _i32, _i32, _i32, _vp, C.POINTER(_vp)]),
     "rag_multi_free": (_i32, [_vp]),
     "rag_multi_ntotal": (_i64, [_vp]),
@@ -114,6 +125,11 @@ class HybridOut(C.Structure):
     """rag_hybrid_out_t: where the search -> fusion -> MMR pipeline leaves its results."""
     _fields_ = [("ids", _vp), ("scores", _vp), ("picked", _vp), ("n_out", _vp), ("fused_rows", _vp),
                 ("fused_scores", _vp), ("fused_sem", _vp), ("fused_bm", _vp), ("n_fused", _vp), ("status", _vp)]
+
+
+class Mx4Store(C.Structure):
+    """rag_mx4_store_t: the caller's buffers of a store of four-bit rows."""
+    _fields_ = [("codes", _vp), ("scales", _vp), ("n", _i64), ("dim", _i32), ("device", _i32)]
 
 
 def _load():

@@ -1,0 +1,32 @@
+// A store of rows kept at four bits: its layout in device memory and the kernels' argument blocks.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace rag {
+
+// A row of `dim` elements is padded with zeros to ks = ceil(dim / 128) blocks of 128 (what one matrix instruction takes
+// along the row).  codes: 64 bytes per block, element 2j of the row in the low half of byte j, 2j + 1 in the high half.
+// scales: one byte per group of 32; the bytes of four consecutive blocks lie together per group column, so that the lane
+// that feeds group column g of a row fetches the scales of four blocks as one dword:
+//     group G of a row (block G / 4, column G % 4)  ->  byte (G / 16) * 16 + (G % 4) * 4 + (G / 4) % 4
+__host__ __device__ __forceinline__ int mx4_blocks(int dim) { return (dim + 127) / 128; }
+__host__ __device__ __forceinline__ int mx4_code_bytes(int dim) { return mx4_blocks(dim) * 64; }
+__host__ __device__ __forceinline__ int mx4_scale_bytes(int dim) { return (mx4_blocks(dim) + 3) / 4 * 16; }
+__host__ __device__ __forceinline__ int mx4_scale_at(int group) { return (group >> 4) * 16 + (group & 3) * 4 + ((group >> 2) & 3); }
+
+constexpr int MX4_MAX_DIM = 8192;          // the query fragments of one matrix tile (2 KiB per block of 128) fit the LDS
+
+// One piece of the grouped product: `nq` queries from q0 against `rows` rows from row0; score (i, r) goes to
+// out[at + i * ld + r].  Written by rag_mx4_plan_groups, read by the kernel.
+struct Mx4Item {
+    long long row0;
+    long long at;
+    int rows;
+    int ld;
+    int q0;
+    int nq;
+};
+static_assert(sizeof(Mx4Item) == 32, "RAG_MX4_ITEM_BYTES");
+
+}  // namespace rag

@@ -1,0 +1,906 @@
+// Rows kept at four bits (e2m1 values, one power-of-two scale per group of 32 consecutive elements: the MX layout):
+// quantising rows as they are written, reading them back, and multiplying them with queries.
+//
+// value(row, i) = sign * T[code & 7] * 2^(scale[i / 32] - 127),  T = {0, 0.5, 1, 1.5, 2, 3, 4, 6};  scale 255: NaN.
+//
+// Products run on the scaled matrix instruction, which reads four-bit values and their scales as they are stored: nothing
+// is unpacked.  Its other operand is eight bits wide (e4m3, scaled per 32 as well), so a query is split into digits first:
+// with 2^E the power of two that brings the largest element of a group of 32 into [8, 16),
+//     x = 2^E * (d0 + d1 / 32 + d2 / 32^2 + ...),   dj a whole number in [-16, 16],
+// and a whole number up to 16 is exact in e4m3.  Each digit is a row of the matrix tile of its own, with the scale
+// 2^(E - 5j), so one instruction multiplies all digits; the digits' sums are added at the end.  fp32 queries take five
+// digits (what is left is at most 2^-24 of the group's largest element), bf16 and fp16 four (at most 2^-19 of it: every
+// element down to 2^-12 (bf16) / 2^-9 (fp16) of the largest one is exact).  Products of such digits with four-bit values
+// are multiples of 1/2 up to 96, which the instruction adds without loss; it adds across groups and to the accumulator in
+// fp32.  One query fills four or five of the tile's sixteen rows, so three (fp32) or four queries cost what one does.
+#include <float.h>
+#include <limits.h>
+#include <math.h>
+#include <stdlib.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "index.h"
+#include "mx4.h"
+#include "topk_keys.h"
+
+namespace rag {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+
+struct Mx4DeviceGuard {
+    int prev = -1;
+    bool ok = true;
+    explicit Mx4DeviceGuard(int dev) {
+        if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+        if (prev != dev) ok = (hipSetDevice(dev) == hipSuccess);
+    }
+    ~Mx4DeviceGuard() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F f) {
+    if constexpr (N > 0) {
+        static_for<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+
+__device__ __forceinline__ float mx4_pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // -126 <= e <= 127
+__device__ __forceinline__ float bf16_f32(unsigned h) { return __uint_as_float(h << 16); }
+__device__ __forceinline__ float f16_f32(unsigned short h) {
+    _Float16 v;
+    __builtin_memcpy(&v, &h, 2);
+    return (float)v;
+}
+// element i of a row of the given type (RAG_MX4_F32 / BF16 / F16)
+__device__ __forceinline__ float mx4_elem(const void* row, int type, long long i) {
+    if (type == RAG_MX4_F32) return static_cast<const float*>(row)[i];
+    const unsigned short h = static_cast<const unsigned short*>(row)[i];
+    return type == RAG_MX4_BF16 ? bf16_f32(h) : f16_f32(h);
+}
+// N (4 or 8) consecutive elements from i on; past `dim` zero.  vec: rows start on 16-byte boundaries.
+template <int N>
+__device__ __forceinline__ void mx4_load(const void* row, int type, int i, int dim, int vec, float* v) {
+    if (vec && i + N <= dim) {
+        if (type == RAG_MX4_F32) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const v4f x = *reinterpret_cast<const v4f*>(static_cast<const float*>(row) + i + j);
+                v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
+            }
+        } else {
+            unsigned w[N / 2];
+            if constexpr (N == 8) {
+                const v4i x = *reinterpret_cast<const v4i*>(static_cast<const unsigned short*>(row) + i);
+                w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+            } else {
+                const v2u x = *reinterpret_cast<const v2u*>(static_cast<const unsigned short*>(row) + i);
+                w[0] = x.x; w[1] = x.y;
+            }
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) {
+                v[2 * j] = type == RAG_MX4_BF16 ? bf16_f32(w[j] & 0xffffu) : f16_f32((unsigned short)w[j]);
+                v[2 * j + 1] = type == RAG_MX4_BF16 ? __uint_as_float(w[j] & 0xffff0000u) : f16_f32((unsigned short)(w[j] >> 16));
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = i + j < dim ? mx4_elem(row, type, i + j) : 0.f;
+}
+
+__device__ __forceinline__ unsigned dpp_max_u32(unsigned v, unsigned o) { return v > o ? v : o; }
+// the largest of |v| (as ordered bits) over each aligned group of 4 / 8 lanes
+__device__ __forceinline__ unsigned quad_max(unsigned v) {
+    v = dpp_max_u32(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+    return dpp_max_u32(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
+}
+__device__ __forceinline__ unsigned oct_max(unsigned v) {
+    v = quad_max(v);
+    return dpp_max_u32(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));   // row_half_mirror
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+// 1 / |x| of one row by one wave: the sum of squares in fp64, rounded once (a zero row keeps its zeros)
+__device__ __forceinline__ float wave_inv_norm(const void* row, int type, int dim, int lane) {
+    double ss = 0.0;
+    for (int i = lane; i < dim; i += 64) {
+        const double x = (double)mx4_elem(row, type, i);
+        ss = fma(x, x, ss);
+    }
+    ss = wave_sum_f64(ss);
+    return ss > 0.0 ? (float)(1.0 / sqrt(ss)) : ss == 0.0 ? 1.f : (float)ss;      // NaN stays NaN
+}
+
+// ------------------------------------------------------------------------------------------------ writing rows
+// Bound by HBM: dim * size bytes in, 0.53 dim bytes out per row.  A lane takes 8 consecutive elements, four lanes a group:
+// loads of 16 (two for fp32) and stores of 4 bytes per lane, both contiguous over the wave.
+struct Mx4WriteArgs {
+    uint8_t* codes;
+    uint8_t* scales;
+    long long n;                 // rows of the store
+    const long long* rows;       // nullptr: row `first + i`
+    int* owner;                  // with rows: owner[r] = 1 + the last i that names row r (mx4_claim_kernel)
+    long long first;
+    long long count;
+    const void* x;
+    long long ldx;               // elements
+    int type, dim, ks, code_ld, scale_ld, normalize, vec;
+    int per_block;               // rows a workgroup takes
+};
+constexpr int MX4_WRITE_ROWS = 64;           // most rows of one workgroup
+
+// A position that is named twice keeps the last of its rows: the highest index wins the claim, whatever the order of arrival.
+__global__ __launch_bounds__(256) void mx4_claim_kernel(const long long* rows, long long count, long long n, int* owner) {
+    const long long i = blockIdx.x * 256ll + threadIdx.x;
+    if (i >= count) return;
+    const long long r = rows[i];
+    if (r >= 0 && r < n) atomicMax(&owner[r], (int)(i + 1));
+}
+
+__global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
+    __shared__ long long s_to[MX4_WRITE_ROWS];
+    __shared__ float s_inv[MX4_WRITE_ROWS];
+    const long long i0 = (long long)blockIdx.x * a.per_block;
+    const int nr = (int)(a.count - i0 < a.per_block ? a.count - i0 : a.per_block);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const size_t esize = a.type == RAG_MX4_F32 ? 4 : 2;
+    if (tid < nr) {
+        long long to = a.first + i0 + tid;
+        if (a.rows) {
+            to = a.rows[i0 + tid];
+            if (to < 0 || to >= a.n) to = -1;
+            else if (a.owner[to] != (int)(i0 + tid + 1)) to = -1;
+            else a.owner[to] = 0;           // only the winner sees its own number here, so no other row is misled by the reset
+        }
+        s_to[tid] = to;
+        s_inv[tid] = 1.f;
+    }
+    __syncthreads();
+    if (a.normalize) {
+        for (int r = tid >> 6; r < nr; r += 4) {
+            const float inv = wave_inv_norm(static_cast<const char*>(a.x) + (size_t)(i0 + r) * a.ldx * esize, a.type, a.dim, lane);
+            if (lane == 0) s_inv[r] = inv;
+        }
+        __syncthreads();
+    }
+    const int upr = a.ks * 16;                                   // units of 8 elements per (padded) row
+    for (int u = tid; u < nr * upr; u += 256) {
+        const int r = u / upr, c = u - r * upr;
+        const long long to = s_to[r];
+        if (to < 0) continue;                                    // uniform over the four lanes of a group
+        float v[8];
+        mx4_load<8>(static_cast<const char*>(a.x) + (size_t)(i0 + r) * a.ldx * esize, a.type, c * 8, a.dim, a.vec, v);
+        unsigned most = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (a.normalize) v[j] *= s_inv[r];
+            const unsigned m = __float_as_uint(v[j]) & 0x7fffffffu;
+            most = m > most ? m : most;
+        }
+        most = quad_max(most);
+        // scale: floor(log2(most)) - 2, one more where most / 2^floor > 1.75 (then 6 is nearer than the 8 that four bits lack)
+        int e = (int)(most >> 23) - 129 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);
+        e = e < -126 ? -126 : e > 125 ? 125 : e;
+        const bool bad = most >= 0x7f800000u;                    // a NaN or an infinity: the group is NaN
+        const float scale = mx4_pow2(e);
+        unsigned w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], scale, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
+        reinterpret_cast<unsigned*>(a.codes + (size_t)to * a.code_ld)[c] = bad ? 0u : w;
+        if ((c & 3) == 0) a.scales[(size_t)to * a.scale_ld + mx4_scale_at(c >> 2)] = bad ? 255 : (uint8_t)(e + 127);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ reading rows
+struct Mx4ReadArgs {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    long long n;
+    const long long* rows;
+    long long count;
+    void* out;                   // [count][dim]
+    int type, dim, ks, code_ld, scale_ld, vec;
+    int per_block;
+};
+
+__device__ __forceinline__ unsigned pack16(int type, float lo, float hi) {
+    if (type == RAG_MX4_BF16) {                                  // four-bit values fit bf16 exactly (subnormal ones round to even)
+        unsigned a = __float_as_uint(lo), b = __float_as_uint(hi);
+        const unsigned ra = lo != lo ? 0x7fc0u : (a + 0x7fffu + ((a >> 16) & 1u)) >> 16;
+        const unsigned rb = hi != hi ? 0x7fc0u : (b + 0x7fffu + ((b >> 16) & 1u)) >> 16;
+        return ra | (rb << 16);
+    }
+    const _Float16 x = (_Float16)lo, y = (_Float16)hi;           // to nearest even
+    unsigned short a, b;
+    __builtin_memcpy(&a, &x, 2);
+    __builtin_memcpy(&b, &y, 2);
+    return (unsigned)a | ((unsigned)b << 16);
+}
+
+__global__ __launch_bounds__(256) void mx4_read_kernel(Mx4ReadArgs a) {
+    const long long i0 = (long long)blockIdx.x * a.per_block;
+    const int nr = (int)(a.count - i0 < a.per_block ? a.count - i0 : a.per_block);
+    const int upr = (a.dim + 7) / 8;
+    for (int u = threadIdx.x; u < nr * upr; u += 256) {
+        const int r = u / upr, c = u - r * upr;
+        const long long from = a.rows[i0 + r];
+        float v[8] = {};
+        if (from >= 0 && from < a.n) {
+            const unsigned w = reinterpret_cast<const unsigned*>(a.codes + (size_t)from * a.code_ld)[c];
+            const unsigned b = a.scales[(size_t)from * a.scale_ld + mx4_scale_at(c >> 2)];
+            const float f = b == 255 ? NAN : b == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(b << 23);
+            v2f p;
+            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0); v[0] = p.x * f; v[1] = p.y * f;
+            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1); v[2] = p.x * f; v[3] = p.y * f;
+            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2); v[4] = p.x * f; v[5] = p.y * f;
+            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3); v[6] = p.x * f; v[7] = p.y * f;
+        }
+        const size_t at = (size_t)(i0 + r) * a.dim + (size_t)c * 8;
+        if (a.vec) {
+            if (a.type == RAG_MX4_F32) {
+                v4f* o = reinterpret_cast<v4f*>(static_cast<float*>(a.out) + at);
+                o[0] = (v4f){v[0], v[1], v[2], v[3]};
+                o[1] = (v4f){v[4], v[5], v[6], v[7]};
+            } else {
+                *reinterpret_cast<v4i*>(static_cast<unsigned short*>(a.out) + at) =
+                    (v4i){(int)pack16(a.type, v[0], v[1]), (int)pack16(a.type, v[2], v[3]), (int)pack16(a.type, v[4], v[5]),
+                          (int)pack16(a.type, v[6], v[7])};
+            }
+        } else {
+            for (int j = 0; j < 8 && c * 8 + j < a.dim; ++j) {
+                if (a.type == RAG_MX4_F32) static_cast<float*>(a.out)[at + j] = v[j];
+                else static_cast<unsigned short*>(a.out)[at + j] = (unsigned short)pack16(a.type, v[j], 0.f);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ products
+struct Mx4ScoreArgs {
+    const uint8_t* codes;        // of the store's first row
+    const uint8_t* scales;
+    const void* q;
+    long long ldq;               // elements
+    int q_type, q_vec, dim, ks, ksu, code_ld, scale_ld, normalize;
+    float* out;
+    // grouped: one workgroup per item
+    const Mx4Item* items;
+    // dense: rows [row0, row0 + rows) cut into slabs, every slab against blocks of QB queries
+    long long row0, rows, slab, out_ld;
+    int nq, nqb;
+};
+
+// Layout of the instruction (checked on the card): lane l, column c = l / 16.  Four-bit operand: row l % 16, elements
+// 32 c .. 32 c + 31 of the block of 128.  Eight-bit operand: row l % 16, bytes 0..15 = elements 16 c .., bytes 16..31 =
+// elements 64 + 16 c ..; scale of lane l (either operand): elements 32 c .. 32 c + 31.  Result register r of lane l:
+// (eight-bit row 4 c + r, four-bit row l % 16).
+//
+// Digit j < 4 of query s of a tile is eight-bit row 4 j + s (result register s, column j); the fifth digit is row 4 s + 3
+// (register 3, column s).
+template <int ND>
+struct Mx4Digits {
+    static constexpr int QPT = ND == 5 ? 3 : 4;        // queries per tile of 16 eight-bit rows
+    static __device__ __forceinline__ int row(int digit, int s) { return digit < 4 ? 4 * digit + s : 4 * s + 3; }
+};
+
+// queries [q0, q0 + nqh) -> digit fragments in LDS.  frag[(block * MT + tile) * 2 + half][lane][16 bytes], then the scales
+// sc[(block / 4) * MT + tile][lane][block % 4], then 1 / |q|.  Blocks past the row's are zero.
+template <int ND, int MT, int NT>
+__device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long long q0, int nqh, uint8_t* frag, uint8_t* sc, float* inv) {
+    constexpr int QPT = Mx4Digits<ND>::QPT;
+    const int tid = threadIdx.x;
+    const v4i zero = {0, 0, 0, 0};
+    const int words = (a.ksu * MT * 2048 + (a.ksu + 3) / 4 * MT * 256) / 16;          // frag and sc are adjacent
+    for (int i = tid; i < words; i += NT) reinterpret_cast<v4i*>(frag)[i] = zero;
+    const size_t esize = a.q_type == RAG_MX4_F32 ? 4 : 2;
+    const char* q = static_cast<const char*>(a.q) + (size_t)q0 * a.ldq * esize;
+    for (int s = tid >> 6; s < MT * QPT; s += NT / 64) {
+        float f = 1.f;
+        if (a.normalize && s < nqh) f = wave_inv_norm(q + (size_t)s * a.ldq * esize, a.q_type, a.dim, tid & 63);
+        if ((tid & 63) == 0) inv[s] = f;
+    }
+    __syncthreads();
+    const int upq = a.ks * 32;                                  // units of 4 elements per query
+    for (int u = tid; u < nqh * upq; u += NT) {
+        const int s = u / upq, c = u - s * upq;
+        float v[4];
+        mx4_load<4>(q + (size_t)s * a.ldq * esize, a.q_type, c * 4, a.dim, a.q_vec, v);
+        unsigned most = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned m = __float_as_uint(v[j]) & 0x7fffffffu;
+            most = m > most ? m : most;
+        }
+        most = oct_max(most);                                   // eight lanes hold a group of 32
+        const bool bad = most >= 0x7f800000u;
+        int e = (int)(most >> 23) - 130;                        // the largest element / 2^e lies in [8, 16)
+        e = e < -100 ? -100 : e;                                // (a group below 2^-97 has its digits cut instead)
+        e = bad ? 0 : e;
+        const float down = mx4_pow2(-e);
+        const int block = c >> 5, in = c & 31;                  // 4 elements `in` of the block
+        const int col = (in >> 2) & 3, half = in >> 4;
+        const int tile = s / QPT, slot = s - tile * QPT;
+        uint8_t* to = frag + (size_t)((block * MT + tile) * 2 + half) * 1024 + col * 256 + (in & 3) * 4;
+        uint8_t* ts = sc + (size_t)((block >> 2) * MT + tile) * 256 + (in >> 3) * 64 + (block & 3);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= down;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            float w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = rintf(v[j]);
+                v[j] = (v[j] - w[j]) * 32.f;                    // both steps exact
+            }
+            int p = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], 0, false);
+            p = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], p, true);
+            if (bad) p = d == 0 ? 0x7f7f7f7f : 0;               // NaN: every score of the query is NaN
+            const int m = Mx4Digits<ND>::row(d, slot);
+            *reinterpret_cast<int*>(to + m * 16) = p;
+            if ((in & 7) == 0) ts[m * 4] = (uint8_t)(127 + e - 5 * d);
+        }
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ float swap_add32(float a, float b) {      // lanes 0..31: a's two halves added; 32..63: b's
+    const v2u r = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false));
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+__device__ __forceinline__ float swap_add16(float a, float b) {      // even columns of 16 lanes: a's pair added; odd: b's
+    const v2u r = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false));
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+// four values, each to be summed over the four columns of lanes: column c is left with the sum of v_c
+__device__ __forceinline__ float columns_sum(float v0, float v1, float v2, float v3) {
+    return swap_add16(swap_add32(v0, v2), swap_add32(v1, v3));
+}
+
+// ND digits, MT tiles of queries, NB blocks of 16 rows per wave, U row blocks of 128 fetched together, NW waves.
+//
+// A wave takes 16 NB rows at a time and keeps the next U blocks of them in flight while the present ones go through the
+// matrix unit; nothing but the query fragments goes through LDS, and there is no barrier after they are staged.
+template <int ND, int MT, int NB, int U, int NW>
+__global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
+    constexpr int QPT = Mx4Digits<ND>::QPT;
+    constexpr int QB = MT * QPT;
+    constexpr int SW = (U + 3) / 4;                             // scale dwords per fetch
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    uint8_t* frag = smem;
+    uint8_t* sc = frag + (size_t)a.ksu * MT * 2048;
+    float* inv = reinterpret_cast<float*>(sc + (size_t)((a.ksu + 3) / 4) * MT * 256);
+
+    long long row0, at, ld;
+    int rows, q0, nqh;
+    if (a.items) {
+        const Mx4Item it = a.items[blockIdx.x];
+        row0 = it.row0; at = it.at; ld = it.ld; rows = it.rows; q0 = it.q0; nqh = it.nq;
+    } else {
+        // consecutive workgroups go to the eight dies in turn: the query blocks of a slab stay on one die, whose L2 then
+        // holds the slab's rows for all of them
+        const long long b = blockIdx.x;
+        long long s = b;
+        int qb = 0;
+        if (a.nqb > 1) {
+            const long long i = b >> 3;
+            s = (i / a.nqb) * 8 + (b & 7);
+            qb = (int)(i % a.nqb);
+        }
+        const long long lo = s * a.slab;
+        if (lo >= a.rows) return;
+        rows = (int)(a.rows - lo < a.slab ? a.rows - lo : a.slab);
+        q0 = qb * QB;
+        nqh = a.nq - q0 < QB ? a.nq - q0 : QB;
+        row0 = a.row0 + lo;
+        at = (long long)q0 * a.out_ld + lo;
+        ld = a.out_ld;
+    }
+    mx4_stage_queries<ND, MT, NW * 64>(a, q0, nqh, frag, sc, inv);
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int n16 = lane & 15, col = lane >> 4;
+    const int tiles = (rows + 16 * NB - 1) / (16 * NB);
+    if (wave >= tiles) return;
+    const int sd = (a.ks + 3) / 4;                              // scale dwords of a lane per row
+
+    struct Buf {
+        v4i w[NB][U];
+        int s[NB][SW];
+    };
+    auto load = [&](Buf& b, int tile, int ks0) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            int r = tile * 16 * NB + nb * 16 + n16;
+            r = r < rows ? r : rows - 1;                        // rows past the end: fetched again, never stored
+            const uint8_t* w = a.codes + (size_t)(row0 + r) * a.code_ld + col * 16;
+            const uint8_t* s = a.scales + (size_t)(row0 + r) * a.scale_ld + col * 4;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = ks0 + u < a.ks ? ks0 + u : a.ks - 1;      // blocks past the row's meet zero digits
+                b.w[nb][u] = *reinterpret_cast<const v4i*>(w + k * 64);
+            }
+#pragma unroll
+            for (int d = 0; d < SW; ++d) {
+                const int k = (ks0 >> 2) + d < sd ? (ks0 >> 2) + d : sd - 1;
+                b.s[nb][d] = *reinterpret_cast<const int*>(s + k * 16);
+            }
+            if constexpr (U < 4) b.s[nb][0] = (int)((unsigned)b.s[nb][0] >> ((ks0 & 3) * 8));
+        }
+    };
+    v4f acc[MT][NB];
+    auto clear = [&]() {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) acc[mt][nb] = (v4f){0.f, 0.f, 0.f, 0.f};
+    };
+    auto multiply = [&](const Buf& b, int ks0) {
+        static_for<U>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const v4i* f = reinterpret_cast<const v4i*>(frag + (size_t)((ks0 + u) * MT + mt) * 2048) + lane;
+                const v4i lo = f[0], hi = f[64];
+                const v8i x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                int xs = reinterpret_cast<const int*>(sc + (size_t)(((ks0 + (U < 4 ? 0 : u)) >> 2) * MT + mt) * 256)[lane];
+                if constexpr (U < 4) xs = (int)((unsigned)xs >> ((ks0 & 3) * 8));
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const v8i y = __builtin_shufflevector(b.w[nb][u], b.w[nb][u], 0, 1, 2, 3, -1, -1, -1, -1);
+                    acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, acc[mt][nb], 0, 4, u & 3, xs, u & 3, b.s[nb][u / 4]);
+                }
+            }
+        });
+    };
+    auto store = [&](int tile) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            // column c of lanes is left with query c of the tile, whose fifth digit lies there already: the order of the
+            // additions is the same for every query, so a score does not depend on what it is computed together with
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const v4f v = acc[mt][nb];
+                const int r = (tile * NB + nb) * 16 + n16, s = mt * QPT + col;
+                float y = columns_sum(v[0], v[1], v[2], ND == 5 ? 0.f : v[3]);
+                if (ND == 5) y += v[3];
+                if (col < QPT && s < nqh && r < rows) a.out[at + (long long)s * ld + r] = y * inv[s];
+            }
+        }
+    };
+
+    Buf x, y;
+    int t = wave, k = 0;
+    load(x, t, 0);
+    clear();
+    auto step = [&](Buf& now, Buf& next) -> bool {              // false: that was the last one
+        int t2 = t, k2 = k + U;
+        if (k2 >= a.ksu) { k2 = 0; t2 += NW; }
+        if (t2 < tiles) load(next, t2, k2);
+        multiply(now, k);
+        if (k2 == 0) {
+            store(t);
+            clear();
+        }
+        t = t2;
+        k = k2;
+        return t2 < tiles;
+    };
+    for (;;) {
+        if (!step(x, y)) break;
+        if (!step(y, x)) break;
+    }
+}
+
+// Which kernel a product takes: from the queries that meet a row, and the row's length.
+struct Mx4Shape {
+    int nd, mt, nb, u, nw, ksu, qb;
+    size_t lds;
+};
+static size_t mx4_lds(int ks, int u, int mt) {
+    const int ksu = (ks + u - 1) / u * u;
+    return (size_t)ksu * mt * 2048 + (size_t)(ksu + 3) / 4 * mt * 256 + (size_t)mt * 4 * sizeof(float);
+}
+static Mx4Shape mx4_shape(int type, int dim, long long nq) {
+    Mx4Shape p = {};
+    const int ks = mx4_blocks(dim);
+    p.nd = type == RAG_MX4_F32 ? 5 : 4;
+    const int qpt = p.nd == 5 ? 3 : 4;
+    const long long need = (nq + qpt - 1) / qpt;
+    auto fetch = [&](int mt) {
+        if (mt <= 2) return ks <= 4 ? ks : ks <= 6 ? 6 : ks <= 8 || (ks & 7) == 0 || (ks & 7) > 4 ? 8 : 4;
+        if (mt == 4) return ks <= 4 ? ks : ks == 6 ? 6 : (ks & 3) == 0 ? 4 : (ks & 1) == 0 ? 2 : 1;
+        return ks <= 4 ? ks : (ks & 3) == 0 ? 4 : (ks & 1) == 0 ? 2 : 1;
+    };
+    p.mt = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8;
+    while (p.mt > 1 && mx4_lds(ks, fetch(p.mt), p.mt) > 160 * 1024) p.mt /= 2;
+    p.u = fetch(p.mt);
+    p.nb = p.mt <= 2 ? 1 : 2;
+    p.nw = p.mt == 8 ? 8 : 4;
+    p.ksu = (ks + p.u - 1) / p.u * p.u;
+    p.qb = p.mt * qpt;
+    p.lds = mx4_lds(ks, p.u, p.mt);
+    return p;
+}
+
+template <int ND, int MT, int NB, int U, int NW>
+static int mx4_launch(const Mx4ScoreArgs& a, long long grid, size_t lds, int device, hipStream_t s) {
+    static bool attr_set[64] = {};          // per device: the attribute belongs to the device's code object
+    auto kern = mx4_scores_kernel<ND, MT, NB, U, NW>;
+    if (lds > 48 * 1024 && !attr_set[device & 63]) {
+        RAG_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        attr_set[device & 63] = true;
+    }
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(NW * 64), lds, s, a);
+    RAG_HIP_CHECK(hipGetLastError());
+    return RAG_OK;
+}
+template <int ND>
+static int mx4_launch_nd(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s) {
+#define MX4_CASE(MT, NB, U, NW) if (p.mt == MT && p.u == U) return mx4_launch<ND, MT, NB, U, NW>(a, grid, p.lds, device, s)
+    MX4_CASE(1, 1, 1, 4); MX4_CASE(1, 1, 2, 4); MX4_CASE(1, 1, 3, 4); MX4_CASE(1, 1, 4, 4); MX4_CASE(1, 1, 6, 4); MX4_CASE(1, 1, 8, 4);
+    MX4_CASE(2, 1, 1, 4); MX4_CASE(2, 1, 2, 4); MX4_CASE(2, 1, 3, 4); MX4_CASE(2, 1, 4, 4); MX4_CASE(2, 1, 6, 4); MX4_CASE(2, 1, 8, 4);
+    MX4_CASE(4, 2, 1, 4); MX4_CASE(4, 2, 2, 4); MX4_CASE(4, 2, 3, 4); MX4_CASE(4, 2, 4, 4); MX4_CASE(4, 2, 6, 4);
+    MX4_CASE(8, 2, 1, 8); MX4_CASE(8, 2, 2, 8); MX4_CASE(8, 2, 3, 8); MX4_CASE(8, 2, 4, 8);
+#undef MX4_CASE
+    return fail(RAG_ERR_INVALID, "internal: no four-bit product kernel for this shape");
+}
+static int mx4_launch_any(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s) {
+    if (grid < 1 || grid > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "four-bit product: grid out of range");
+    return p.nd == 5 ? mx4_launch_nd<5>(p, a, grid, device, s) : mx4_launch_nd<4>(p, a, grid, device, s);
+}
+
+static int mx4_check_store(const rag_mx4_store_t* st) {
+    if (!st) return fail(RAG_ERR_INVALID, "store is NULL");
+    if (st->dim < 1 || st->dim > MX4_MAX_DIM) return fail(RAG_ERR_INVALID, "dim must be in [1, " + std::to_string(MX4_MAX_DIM) + "]");
+    if (st->n < 0 || st->n > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "a store holds 0 to 2^31 - 1 rows");
+    if (st->n > 0 && (!st->codes || !st->scales)) return fail(RAG_ERR_INVALID, "store without buffers");
+    if ((reinterpret_cast<uintptr_t>(st->codes) & 15) || (reinterpret_cast<uintptr_t>(st->scales) & 15))
+        return fail(RAG_ERR_INVALID, "the store's buffers must lie on 16-byte boundaries");
+    return RAG_OK;
+}
+static int mx4_check_type(int type) {
+    if (type != RAG_MX4_F32 && type != RAG_MX4_BF16 && type != RAG_MX4_F16) return fail(RAG_ERR_INVALID, "unknown element type");
+    return RAG_OK;
+}
+static size_t mx4_esize(int type) { return type == RAG_MX4_F32 ? 4 : 2; }
+static int mx4_aligned(const void* p, long long ld, int type) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (size_t)ld * mx4_esize(type) % 16 == 0;
+}
+static Mx4ScoreArgs mx4_score_args(const rag_mx4_store_t* st, const Mx4Shape& p, const void* q, int q_type, long long ldq, int normalize, float* out) {
+    Mx4ScoreArgs a = {};
+    a.codes = static_cast<const uint8_t*>(st->codes);
+    a.scales = static_cast<const uint8_t*>(st->scales);
+    a.q = q;
+    a.ldq = ldq;
+    a.q_type = q_type;
+    a.q_vec = mx4_aligned(q, ldq, q_type);
+    a.dim = st->dim;
+    a.ks = mx4_blocks(st->dim);
+    a.ksu = p.ksu;
+    a.code_ld = mx4_code_bytes(st->dim);
+    a.scale_ld = mx4_scale_bytes(st->dim);
+    a.normalize = normalize;
+    a.out = out;
+    return a;
+}
+
+// scores of rows [row0, row0 + rows) (checked by the caller)
+static int mx4_scores(const rag_mx4_store_t* st, long long row0, long long rows, long long nq, const void* q, int q_type, long long ldq,
+                      int normalize, float* out, long long out_ld, hipStream_t s) {
+    const Mx4Shape p = mx4_shape(q_type, st->dim, nq);
+    Mx4ScoreArgs a = mx4_score_args(st, p, q, q_type, ldq, normalize, out);
+    a.row0 = row0;
+    a.rows = rows;
+    a.out_ld = out_ld;
+    a.nq = (int)nq;
+    a.nqb = (int)((nq + p.qb - 1) / p.qb);
+    const long long unit = 16LL * p.nb * p.nw;                  // rows of one step of a workgroup
+    const long long units = (rows + unit - 1) / unit;
+    const long long want = std::max<long long>(1, (p.mt == 8 ? 2048 : 1024) / a.nqb);     // slabs
+    a.slab = (units + want - 1) / want * unit;
+    a.slab = std::min<long long>(a.slab, 1LL << 30);
+    const long long slabs = (rows + a.slab - 1) / a.slab;
+    const long long grid = a.nqb > 1 ? (slabs + 7) / 8 * 8 * a.nqb : slabs;
+    return mx4_launch_any(p, a, grid, st->device, s);
+}
+
+int direct_select_segments(long long nq, long long n_row, long long seg_rows, int k, float min_score, const uint8_t* mask,
+                           const long long* row_ids, long long id_base, const float* scores, float* D, long long* I, long long out_stride,
+                           const float* floor, long long floor_stride, hipStream_t s);   // direct_topk.hip
+int merge_lists_device(int nlists, long long nq, int k, const float* D_dev, long long d_list_stride, const long long* I_dev,
+                       long long i_list_stride, float* D_out, long long* I_out, u64* keys, hipStream_t s);      // api.hip
+void launch_fill_results(float* D, long long* I, long long n, hipStream_t s);                // api.hip
+
+__global__ void mx4_copy_lists_kernel(const float* D, const long long* I, long long n, float* Dto, long long* Ito) {
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+        Dto[i] = D[i];
+        Ito[i] = I[i];
+    }
+}
+
+__global__ void mx4_and_masks_kernel(const uint8_t* a, const uint8_t* b, long long n, uint8_t* out) {
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x)
+        out[i] = (a[i] != 0 && b[i] != 0) ? 1 : 0;
+}
+
+// A search walks the rows in spans whose scores fit 256 MiB: score matrix, the k best of every 32768 rows, merge.
+constexpr long long MX4_SEG = 32768;
+struct Mx4Plan {
+    long long qc, span;          // queries and rows of one step
+    size_t scores, d, i, keys, mask;     // bytes of the workspace's parts
+    size_t total() const { return scores + d + i + keys + mask; }
+};
+static Mx4Plan mx4_plan(long long n, long long nq, int k) {
+    Mx4Plan p;
+    const long long segs = std::max<long long>(1, (n + MX4_SEG - 1) / MX4_SEG);
+    p.qc = std::min<long long>(std::max<long long>(nq, 1), 512);
+    p.span = std::max<long long>(1, std::min<long long>(std::min<long long>(segs, 256), (256LL << 20) / (p.qc * MX4_SEG * 4)));
+    // the merge reads (span + 1) lists of k keys per query
+    while (p.span > 1 && (p.span + 1) * p.qc * k > (16LL << 20)) p.span /= 2;
+    auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    p.scores = al((size_t)p.qc * std::min<long long>(std::max<long long>(n, 1), p.span * MX4_SEG) * sizeof(float));
+    p.d = al((size_t)(p.span + 1) * p.qc * k * sizeof(float));
+    p.i = al((size_t)(p.span + 1) * p.qc * k * sizeof(long long));
+    p.keys = al((size_t)(p.span + 1) * p.qc * k * sizeof(u64));
+    p.mask = al((size_t)std::max<long long>(n, 1));
+    return p;
+}
+
+}  // namespace rag
+
+using namespace rag;
+
+extern "C" {
+
+int rag_mx4_layout(int dim, int64_t* code_bytes, int64_t* scale_bytes) {
+    if (dim < 1 || dim > MX4_MAX_DIM) return fail(RAG_ERR_INVALID, "dim must be in [1, " + std::to_string(MX4_MAX_DIM) + "]");
+    if (!code_bytes || !scale_bytes) return fail(RAG_ERR_INVALID, "NULL output");
+    *code_bytes = mx4_code_bytes(dim);
+    *scale_bytes = mx4_scale_bytes(dim);
+    return RAG_OK;
+}
+
+int rag_mx4_write_device(const rag_mx4_store_t* st, int64_t first, const int64_t* rows_dev, int32_t* owner_dev, int64_t count,
+                         const void* x_dev, int x_type, int64_t x_stride, int normalize, void* stream) {
+    if (int rc = mx4_check_store(st)) return rc;
+    if (int rc = mx4_check_type(x_type)) return rc;
+    if (count < 0 || count >= 0x7fffffffLL) return fail(RAG_ERR_INVALID, "count out of range");
+    if (count == 0) return RAG_OK;
+    if (!x_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
+    if (x_stride < st->dim) return fail(RAG_ERR_INVALID, "x_stride smaller than dim");
+    if ((reinterpret_cast<uintptr_t>(x_dev) & (mx4_esize(x_type) - 1))) return fail(RAG_ERR_INVALID, "x is not aligned to its elements");
+    if (rows_dev) {
+        if (!owner_dev) return fail(RAG_ERR_INVALID, "positions need the store's owner array");
+        if (st->n == 0) return RAG_OK;                  // every position lies outside
+    } else if (first < 0 || first > st->n || count > st->n - first) {
+        return fail(RAG_ERR_INVALID, "rows [first, first + count) do not lie inside the store");
+    }
+    Mx4DeviceGuard g(st->device);
+    if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    Mx4WriteArgs a = {};
+    a.codes = static_cast<uint8_t*>(st->codes);
+    a.scales = static_cast<uint8_t*>(st->scales);
+    a.n = st->n;
+    a.rows = reinterpret_cast<const long long*>(rows_dev);
+    a.owner = owner_dev;
+    a.first = first;
+    a.count = count;
+    a.x = x_dev;
+    a.ldx = x_stride;
+    a.type = x_type;
+    a.dim = st->dim;
+    a.ks = mx4_blocks(st->dim);
+    a.code_ld = mx4_code_bytes(st->dim);
+    a.scale_ld = mx4_scale_bytes(st->dim);
+    a.normalize = normalize ? 1 : 0;
+    a.vec = mx4_aligned(x_dev, x_stride, x_type);
+    a.per_block = std::max(1, std::min(MX4_WRITE_ROWS, 1024 / (a.ks * 16)));
+    if (rows_dev) {
+        hipLaunchKernelGGL(mx4_claim_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, a.rows, (long long)count, a.n, a.owner);
+        RAG_HIP_CHECK(hipGetLastError());
+    }
+    hipLaunchKernelGGL(mx4_write_kernel, dim3((unsigned)((count + a.per_block - 1) / a.per_block)), dim3(256), 0, s, a);
+    RAG_HIP_CHECK(hipGetLastError());
+    return RAG_OK;
+}
+
+int rag_mx4_read_device(const rag_mx4_store_t* st, const int64_t* rows_dev, int64_t count, void* out_dev, int out_type, void* stream) {
+    if (int rc = mx4_check_store(st)) return rc;
+    if (int rc = mx4_check_type(out_type)) return rc;
+    if (count < 0 || count >= 0x7fffffffLL) return fail(RAG_ERR_INVALID, "count out of range");
+    if (count == 0) return RAG_OK;
+    if (!rows_dev || !out_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
+    if ((reinterpret_cast<uintptr_t>(out_dev) & (mx4_esize(out_type) - 1))) return fail(RAG_ERR_INVALID, "out is not aligned to its elements");
+    Mx4DeviceGuard g(st->device);
+    if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
+    Mx4ReadArgs a = {};
+    a.codes = static_cast<const uint8_t*>(st->codes);
+    a.scales = static_cast<const uint8_t*>(st->scales);
+    a.n = st->n;
+    a.rows = reinterpret_cast<const long long*>(rows_dev);
+    a.count = count;
+    a.out = out_dev;
+    a.type = out_type;
+    a.dim = st->dim;
+    a.ks = mx4_blocks(st->dim);
+    a.code_ld = mx4_code_bytes(st->dim);
+    a.scale_ld = mx4_scale_bytes(st->dim);
+    a.vec = st->dim % 8 == 0 && mx4_aligned(out_dev, st->dim, out_type);
+    a.per_block = std::max(1, std::min(MX4_WRITE_ROWS, 1024 / ((st->dim + 7) / 8)));
+    hipLaunchKernelGGL(mx4_read_kernel, dim3((unsigned)((count + a.per_block - 1) / a.per_block)), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), a);
+    RAG_HIP_CHECK(hipGetLastError());
+    return RAG_OK;
+}
+
+static int mx4_check_queries(const rag_mx4_store_t* st, int64_t nq, const void* q_dev, int q_type, int64_t q_stride) {
+    if (int rc = mx4_check_store(st)) return rc;
+    if (int rc = mx4_check_type(q_type)) return rc;
+    if (nq < 0 || nq > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "nq out of range");
+    if (nq > 0 && !q_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
+    if (nq > 0 && q_stride < st->dim) return fail(RAG_ERR_INVALID, "q_stride smaller than dim");
+    if ((reinterpret_cast<uintptr_t>(q_dev) & (mx4_esize(q_type) - 1))) return fail(RAG_ERR_INVALID, "q is not aligned to its elements");
+    return RAG_OK;
+}
+
+int rag_mx4_scores_device(const rag_mx4_store_t* st, int64_t row_begin, int64_t row_end, int64_t nq, const void* q_dev, int q_type,
+                          int64_t q_stride, int normalize, float* out_dev, int64_t out_stride, void* stream) {
+    if (int rc = mx4_check_queries(st, nq, q_dev, q_type, q_stride)) return rc;
+    if (row_begin < 0 || row_end < row_begin || row_end > st->n) return fail(RAG_ERR_INVALID, "rows [row_begin, row_end) do not lie inside the store");
+    const long long rows = row_end - row_begin;
+    if (nq == 0 || rows == 0) return RAG_OK;
+    if (!out_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
+    if (out_stride < rows) return fail(RAG_ERR_INVALID, "out_stride smaller than the number of rows");
+    Mx4DeviceGuard g(st->device);
+    if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
+    return mx4_scores(st, row_begin, rows, nq, q_dev, q_type, q_stride, normalize ? 1 : 0, out_dev, out_stride, static_cast<hipStream_t>(stream));
+}
+
+int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngroups, const int64_t* groups, int64_t max_items,
+                        void* items_out, int64_t* n_items, int64_t* out_begin, int64_t* total, int32_t* widest) {
+    if (dim < 1 || dim > MX4_MAX_DIM) return fail(RAG_ERR_INVALID, "dim must be in [1, " + std::to_string(MX4_MAX_DIM) + "]");
+    if (int rc = mx4_check_type(q_type)) return rc;
+    if (ngroups < 0 || nq < 0 || nq > 0x7fffffffLL || n < 0 || n > 0x7fffffffLL || max_items < 0) return fail(RAG_ERR_INVALID, "size out of range");
+    if ((ngroups > 0 && !groups) || !n_items || !total || !widest || (max_items > 0 && !items_out)) return fail(RAG_ERR_INVALID, "NULL buffer");
+    long long most_q = 0, sum = 0;
+    __int128 pairs = 0;
+    for (long long g = 0; g < ngroups; ++g) {
+        const int64_t* d = groups + 4 * g;
+        if (d[0] < 0 || d[1] < d[0] || d[1] > nq) return fail(RAG_ERR_INVALID, "group " + std::to_string(g) + ": queries do not lie inside [0, nq)");
+        if (d[2] < 0 || d[3] < d[2] || d[3] > n) return fail(RAG_ERR_INVALID, "group " + std::to_string(g) + ": rows do not lie inside the store");
+        if (out_begin) out_begin[g] = sum;
+        pairs += (__int128)(d[1] - d[0]) * (d[3] - d[2]);
+        if (pairs > (__int128)1 << 60) return fail(RAG_ERR_INVALID, "too many scores");
+        sum = (long long)pairs;
+        if (d[3] > d[2]) most_q = std::max<long long>(most_q, d[1] - d[0]);
+    }
+    *total = sum;
+    *widest = (int32_t)most_q;
+    const Mx4Shape p = mx4_shape(q_type, dim, std::max<long long>(most_q, 1));
+    // rows of an item: enough items to fill the chip several times over, each long enough to pay for staging its queries
+    long long work = 0;
+    for (long long g = 0; g < ngroups; ++g)
+        work += (groups[4 * g + 1] - groups[4 * g] + p.qb - 1) / p.qb * (groups[4 * g + 3] - groups[4 * g + 2]);
+    const long long unit = 16LL * p.nb * p.nw;
+    const long long part = std::max<long long>(2 * unit, std::min<long long>(8192, (work / 2048 + unit - 1) / unit * unit));
+    long long m = 0;
+    Mx4Item* items = static_cast<Mx4Item*>(items_out);
+    long long at = 0;
+    for (long long g = 0; g < ngroups; ++g) {
+        const int64_t* d = groups + 4 * g;
+        const long long gq = d[1] - d[0], gr = d[3] - d[2];
+        for (long long r = 0; r < gr && gq > 0; r += part)
+            for (long long q = 0; q < gq; q += p.qb, ++m)
+                if (m < max_items) {
+                    Mx4Item it;
+                    it.row0 = d[2] + r;
+                    it.at = at + q * gr + r;
+                    it.rows = (int)std::min(part, gr - r);
+                    it.ld = (int)gr;
+                    it.q0 = (int)(d[0] + q);
+                    it.nq = (int)std::min<long long>(p.qb, gq - q);
+                    items[m] = it;
+                }
+        at += gq * gr;
+    }
+    *n_items = m;
+    return RAG_OK;
+}
+
+int rag_mx4_scores_grouped_device(const rag_mx4_store_t* st, int64_t nq, const void* q_dev, int q_type, int64_t q_stride, int normalize,
+                                  const void* items_dev, int64_t n_items, int32_t widest, float* out_dev, void* stream) {
+    if (int rc = mx4_check_queries(st, nq, q_dev, q_type, q_stride)) return rc;
+    if (n_items < 0 || n_items > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "n_items out of range");
+    if (n_items == 0) return RAG_OK;
+    if (nq == 0 || !items_dev || !out_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
+    if ((reinterpret_cast<uintptr_t>(items_dev) & 15)) return fail(RAG_ERR_INVALID, "items must lie on a 16-byte boundary");
+    if (widest < 1 || widest > nq) return fail(RAG_ERR_INVALID, "widest is not what rag_mx4_plan_groups gave for these queries");
+    Mx4DeviceGuard g(st->device);
+    if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
+    const Mx4Shape p = mx4_shape(q_type, st->dim, widest);
+    Mx4ScoreArgs a = mx4_score_args(st, p, q_dev, q_type, q_stride, normalize ? 1 : 0, out_dev);
+    a.items = static_cast<const Mx4Item*>(items_dev);
+    a.nq = (int)nq;
+    return mx4_launch_any(p, a, n_items, st->device, static_cast<hipStream_t>(stream));
+}
+
+int64_t rag_mx4_search_workspace(int64_t n, int64_t nq, int k) {
+    if (n < 0 || nq < 0 || k < 1 || k > 1024) return -1;
+    return (int64_t)mx4_plan(n, nq, k).total();
+}
+
+int rag_mx4_search_device(const rag_mx4_store_t* st, int64_t nq, const void* q_dev, int q_type, int64_t q_stride, int normalize, int k,
+                          float min_score, const uint8_t* row_mask_dev, const uint8_t* active_dev, float* D_dev, int64_t* I_dev, void* workspace_dev,
+                          int64_t workspace_bytes, void* stream) {
+    if (int rc = mx4_check_queries(st, nq, q_dev, q_type, q_stride)) return rc;
+    if (k < 1 || k > 1024) return fail(RAG_ERR_INVALID, "k must be in [1, 1024]");
+    if (min_score != min_score) return fail(RAG_ERR_INVALID, "min_score is NaN");
+    if (nq == 0) return RAG_OK;
+    if (!D_dev || !I_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
+    Mx4DeviceGuard g(st->device);
+    if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    long long* I = reinterpret_cast<long long*>(I_dev);
+    if (st->n == 0) {
+        launch_fill_results(D_dev, I, (long long)nq * k, s);
+        RAG_HIP_CHECK(hipGetLastError());
+        return RAG_OK;
+    }
+    const Mx4Plan p = mx4_plan(st->n, nq, k);
+    if (!workspace_dev || (reinterpret_cast<uintptr_t>(workspace_dev) & 255) || workspace_bytes < (int64_t)p.total())
+        return fail(RAG_ERR_INVALID, "workspace: " + std::to_string(p.total()) + " bytes on a 256-byte boundary are needed");
+    char* w = static_cast<char*>(workspace_dev);
+    float* scores = reinterpret_cast<float*>(w);
+    float* Dl = reinterpret_cast<float*>(w + p.scores);
+    long long* Il = reinterpret_cast<long long*>(w + p.scores + p.d);
+    u64* keys = reinterpret_cast<u64*>(w + p.scores + p.d + p.i);
+    const uint8_t* mask = row_mask_dev ? row_mask_dev : active_dev;
+    if (row_mask_dev && active_dev) {
+        uint8_t* both = reinterpret_cast<uint8_t*>(w + p.scores + p.d + p.i + p.keys);
+        hipLaunchKernelGGL(mx4_and_masks_kernel, dim3((unsigned)std::min<long long>(4096, (st->n + 255) / 256)), dim3(256), 0, s, row_mask_dev,
+                           active_dev, (long long)st->n, both);
+        RAG_HIP_CHECK(hipGetLastError());
+        mask = both;
+    }
+    for (long long q0 = 0; q0 < nq; q0 += p.qc) {
+        const long long qc = std::min<long long>(p.qc, nq - q0);
+        const long long lists = qc * k;                       // hits of one list per query
+        const char* q = static_cast<const char*>(q_dev) + (size_t)q0 * q_stride * mx4_esize(q_type);
+        // list 0 is the answer so far; its k-th score is a floor for the rows behind it
+        launch_fill_results(Dl, Il, lists, s);
+        for (long long lo = 0; lo < st->n; lo += p.span * MX4_SEG) {
+            const long long rows = std::min<long long>(p.span * MX4_SEG, st->n - lo);
+            const int segs = (int)((rows + MX4_SEG - 1) / MX4_SEG);
+            if (int rc = mx4_scores(st, lo, rows, qc, q, q_type, q_stride, normalize ? 1 : 0, scores, rows, s)) return rc;
+            if (int rc = direct_select_segments(qc, rows, MX4_SEG, k, min_score, mask ? mask + lo : nullptr, nullptr, lo, scores,
+                                                Dl + lists, Il + lists, lists, lo > 0 ? Dl + (k - 1) : nullptr, k, s))
+                return rc;
+            float* Do = D_dev + (size_t)q0 * k;
+            long long* Io = I + (size_t)q0 * k;
+            if (int rc = merge_lists_device(segs + 1, qc, k, Dl, lists, Il, lists, Do, Io, keys, s)) return rc;
+            if (lo + rows < st->n) {
+                hipLaunchKernelGGL(mx4_copy_lists_kernel, dim3((unsigned)std::min<long long>(256, (lists + 255) / 256)), dim3(256), 0, s, Do, Io,
+                                   lists, Dl, Il);
+                RAG_HIP_CHECK(hipGetLastError());
+            }
+        }
+    }
+    return RAG_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,379 @@
+"""Vector index whose rows are kept at four bits: what the reference's ``quantization_config`` asks its server for
+(vector_db/search_optimizer.py:51,130), without the originals beside it.
+
+``QuantizedIndex`` has the method names of ``DeviceIndex`` (add, search, reconstruct, set_active, make_filter, save / load)
+and two products of its own, ``scores`` and ``scores_grouped``.  A row takes 0.53 bytes per element -- four-bit values (e2m1)
+with one power-of-two scale per 32 elements -- and every answer is exact for the rows as they are stored.  The buffers are
+torch tensors; every device call runs on torch's current stream of the index's device, allocates through torch only, and may be
+captured into a CUDA graph.  Calls that write the index and calls that use it are ordered by the caller's streams.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import os
+from typing import Optional, Tuple
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .index import FLT_MAX, MAX_K, DeviceFilter, _device_mask_ptr, _is_torch_cuda, _ptr
+
+MAX_DIM = 8192
+
+
+_TYPES = {torch.float32: _lib.MX4_F32, torch.bfloat16: _lib.MX4_BF16, torch.float16: _lib.MX4_F16}
+
+
+def _type_of(dtype) -> int:
+    kind = _TYPES.get(dtype)
+    if kind is None:
+        raise ValueError(f"expected float32, bfloat16 or float16, got {dtype}")
+    return kind
+
+
+class _Kept:
+    """Device tensors that calls on several streams may use: a stream other than the one they were made on is made
+    known to torch's allocator, so that their memory is not handed out again before that stream is done with them."""
+
+    def __init__(self, device: int):
+        self.device = device
+        self.made_on = torch._C._cuda_getCurrentRawStream(device)
+        self.tensors = []
+
+    def stream(self) -> int:
+        """The current stream, as the C ABI takes it."""
+        raw = torch._C._cuda_getCurrentRawStream(self.device)
+        if raw != self.made_on:
+            s = torch.cuda.current_stream(self.device)
+            for t in self.tensors:
+                t.record_stream(s)
+        return raw
+
+
+class GroupPlan:
+    """Ragged groups of queries and rows, checked and cut into pieces for the device (``rag_mx4_plan_groups``).
+    ``total``: scores of all groups; ``out_begin[g]``: where those of group g start; ``shapes[g]``: (queries, rows)."""
+
+    def __init__(self, groups, nq: int, n: int, dim: int, dtype, device: int):
+        g = np.ascontiguousarray(groups, dtype=np.int64)
+        if g.size == 0:
+            g = g.reshape(0, 4)
+        if g.ndim != 2 or g.shape[1] != 4:
+            raise ValueError("groups must be [n, 4]: query begin, query end, row begin, row end")
+        self.nq, self.n, self.type, self.device = int(nq), int(n), _type_of(dtype), int(device)
+        self.shapes = np.stack([g[:, 1] - g[:, 0], g[:, 3] - g[:, 2]], 1)
+        self.out_begin = np.zeros(g.shape[0], dtype=np.int64)
+        count, total, widest = C.c_int64(0), C.c_int64(0), C.c_int32(0)
+
+        def plan(room, ptr):
+            check(lib.rag_mx4_plan_groups(int(dim), self.type, self.nq, self.n, g.shape[0], _ptr(g), room, ptr, C.byref(count),
+                                          _ptr(self.out_begin), C.byref(total), C.byref(widest)))
+        room = 4 * g.shape[0] + 64
+        staging = torch.empty((room, _lib.MX4_ITEM_BYTES), dtype=torch.uint8, pin_memory=True)
+        plan(room, C.c_void_p(staging.data_ptr()))
+        if count.value > room:
+            room = count.value
+            staging = torch.empty((room, _lib.MX4_ITEM_BYTES), dtype=torch.uint8, pin_memory=True)
+            plan(room, C.c_void_p(staging.data_ptr()))
+        self.total, self.widest, self.n_items = int(total.value), int(widest.value), int(count.value)
+        self._kept = _Kept(self.device)
+        self.items = staging[:self.n_items].to(torch.device("cuda", self.device), non_blocking=True)
+        self._kept.tensors = [self.items]
+
+    def split(self, scores):
+        """The flat result of ``scores_grouped`` as one [queries, rows] view per group."""
+        return [scores[b:b + q * r].view(q, r) for b, (q, r) in zip(self.out_begin.tolist(), self.shapes.tolist())]
+
+
+class QuantizedIndex:
+    """metric: 'ip' | 'cosine' (rows are divided by their norm when written, queries when scored)."""
+
+    kind = "mx4"
+
+    def __init__(self, dim: int, metric: str = "cosine", device: int = 0, capacity: int = 0):
+        if metric not in ("ip", "dot", "cosine"):
+            raise ValueError(f"unknown metric {metric!r}")
+        self.dim, self.metric, self.device = int(dim), metric, int(device)
+        code_bytes, scale_bytes = C.c_int64(0), C.c_int64(0)
+        check(lib.rag_mx4_layout(self.dim, C.byref(code_bytes), C.byref(scale_bytes)))
+        self._code_bytes, self._scale_bytes = int(code_bytes.value), int(scale_bytes.value)
+        n = C.c_int(0)
+        check(lib.rag_device_count(C.byref(n)))
+        if not 0 <= self.device < n.value:
+            raise ValueError(f"no device {self.device}")
+        self._kept = _Kept(self.device)
+        self._dev = torch.device("cuda", self.device)
+        self._normalize = 1 if metric == "cosine" else 0
+        self._n = 0
+        self._codes = self._scales = self._owner = self._active = None
+        self.last_path = "none"
+        self._renew()
+        self.reserve(int(capacity))
+
+    # ------------------------------------------------------------------ lifetime
+    def close(self) -> None:
+        self._n = 0
+        self._codes = self._scales = self._owner = self._active = None
+        self._renew()
+
+    def __len__(self) -> int:
+        return self._n
+
+    @property
+    def ntotal(self) -> int:
+        return self._n
+
+    def _renew(self) -> None:
+        """After a change of the buffers or of the number of rows: what the C ABI is told about them."""
+        self._st = _lib.Mx4Store()
+        if self._codes is not None:
+            self._st.codes, self._st.scales = self._codes.data_ptr(), self._scales.data_ptr()
+        self._st.n, self._st.dim, self._st.device = self._n, self.dim, self.device
+        self._st_ref = C.byref(self._st)
+        self._kept.tensors = [t for t in (self._codes, self._scales, self._owner, self._active) if t is not None]
+
+    def reserve(self, nrows: int) -> None:
+        """Room for ``nrows`` rows, so that adds up to there move nothing."""
+        have = 0 if self._codes is None else self._codes.shape[0]
+        if nrows <= have:
+            return
+        dev = self._dev
+        made = _Kept(self.device)
+        codes = torch.zeros((nrows, self._code_bytes), dtype=torch.uint8, device=dev)
+        scales = torch.zeros((nrows, self._scale_bytes), dtype=torch.uint8, device=dev)
+        owner = torch.zeros((nrows,), dtype=torch.int32, device=dev)
+        if self._n:
+            codes[:self._n] = self._codes[:self._n]
+            scales[:self._n] = self._scales[:self._n]
+        self._codes, self._scales, self._owner, self._kept = codes, scales, owner, made
+        self._renew()
+
+    # -------------------------------------------------------------------- ingest
+    def _rows_in(self, x, what="rows"):
+        """x as a device matrix [n, dim] whose rows may lie apart (inner stride 1)."""
+        if _is_torch_cuda(x):
+            if x.device.index != self.device:
+                raise ValueError("tensor is on another device than the index")
+            _type_of(x.dtype)
+        else:
+            x = torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32))
+        if x.dim() == 1:
+            x = x[None, :]
+        if x.dim() != 2 or x.shape[1] != self.dim:
+            raise ValueError(f"expected {what} [n, {self.dim}], got {tuple(x.shape)}")
+        if not x.is_cuda:
+            x = x.to(self._dev)
+        if x.shape[0] and (x.stride(1) != 1 and self.dim > 1 or x.stride(0) < self.dim and x.shape[0] > 1):
+            x = x.contiguous()
+        return x, max(x.stride(0), self.dim)
+
+    def add(self, x) -> None:
+        """Append rows (numpy, or a CUDA tensor in float32, bfloat16 or float16), quantised as they are written."""
+        x, ld = self._rows_in(x)
+        first, count = self._n, x.shape[0]
+        if count == 0:
+            return
+        have = 0 if self._codes is None else self._codes.shape[0]
+        if first + count > have:
+            self.reserve(max(first + count, have + have // 2))
+        self._n = first + count
+        if self._active is not None:
+            self._active = torch.cat([self._active, torch.ones((count,), dtype=torch.uint8, device=self._dev)])
+        self._renew()
+        self._write(first, None, count, x, ld)
+
+    def write(self, rows, x) -> None:
+        """Replace rows.  ``rows``: the first of consecutive positions (int), or one position per row of ``x`` (numpy, or
+        a CUDA int64 tensor); a position outside the index is skipped, of several rows for one position the last is kept."""
+        x, ld = self._rows_in(x)
+        if isinstance(rows, (int, np.integer)):
+            if not 0 <= int(rows) <= self._n - x.shape[0]:
+                raise ValueError("the rows do not lie inside the index")
+            self._write(int(rows), None, x.shape[0], x, ld)
+            return
+        at = self._positions(rows)
+        if at.numel() != x.shape[0]:
+            raise ValueError("one position per row")
+        self._write(0, at, x.shape[0], x, ld)
+
+    def _positions(self, rows):
+        if _is_torch_cuda(rows):
+            if rows.dtype != torch.int64 or rows.device.index != self.device:
+                raise ValueError("positions must be an int64 tensor on the index's device")
+            return rows.reshape(-1).contiguous()
+        return torch.from_numpy(np.ascontiguousarray(rows, dtype=np.int64).reshape(-1)).to(self._dev)
+
+    def _write(self, first, at, count, x, ld):
+        if count == 0 or self._n == 0:
+            return
+        check(lib.rag_mx4_write_device(self._st_ref, first, None if at is None else at.data_ptr(),
+                                       None if at is None else self._owner.data_ptr(), count, x.data_ptr(), _type_of(x.dtype), ld,
+                                       self._normalize, self._kept.stream()))
+
+    @classmethod
+    def from_packed(cls, codes, scales, dim: int, metric: str = "ip", device: Optional[int] = None) -> "QuantizedIndex":
+        """An index over rows that are quantised already (a checkpoint in the MX layout).  ``codes`` uint8
+        [n, 16 * ceil(dim / 32)]: element 2j in the low, 2j + 1 in the high half of byte j; ``scales`` uint8 [n, ceil(dim / 32)].
+        Both are copied; elements behind ``dim`` are set to zero."""
+        groups = (int(dim) + 31) // 32
+        codes = codes if isinstance(codes, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(codes, dtype=np.uint8))
+        scales = scales if isinstance(scales, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(scales, dtype=np.uint8))
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2 \
+                or codes.shape[0] != scales.shape[0] or codes.shape[1] != 16 * groups or scales.shape[1] != groups:
+            raise ValueError(f"expected uint8 codes [n, {16 * groups}] and scales [n, {groups}]")
+        if device is None:
+            device = codes.device.index if codes.is_cuda else 0
+        n = codes.shape[0]
+        self = cls(dim, metric=metric, device=device, capacity=n)
+        if n:
+            dev = self._dev
+            self._codes[:, :16 * groups] = codes.to(dev)
+            if self.dim % 32:
+                self._codes[:, (self.dim + 1) // 2:] = 0
+                if self.dim % 2:
+                    self._codes[:, self.dim // 2] &= 15
+            self._scales[:, torch.from_numpy(_scale_places(groups)).to(dev)] = scales.to(dev)
+            self._n = n
+            self._renew()
+        return self
+
+    def packed(self) -> Tuple[object, object]:
+        """(codes, scales) of all rows as ``from_packed`` takes them, copied."""
+        groups = (self.dim + 31) // 32
+        if self._n == 0:
+            dev = self._dev
+            return (torch.empty((0, 16 * groups), dtype=torch.uint8, device=dev), torch.empty((0, groups), dtype=torch.uint8, device=dev))
+        places = torch.from_numpy(_scale_places(groups)).to(self._codes.device)
+        return self._codes[:self._n, :16 * groups].clone(), self._scales[:self._n][:, places]
+
+    def set_active(self, rows, active: bool) -> None:
+        """Hide rows from every search, or show them again (vector_db/qdrant_client.py:826-883)."""
+        rows = np.ascontiguousarray(rows, dtype=np.int64).reshape(-1)
+        if rows.size and (rows.min() < 0 or rows.max() >= self._n):
+            raise ValueError("row position out of range")
+        if rows.size == 0:
+            return
+        if self._active is None:
+            if active:
+                return
+            self._active = torch.ones((self._n,), dtype=torch.uint8, device=self._dev)
+            self._renew()
+        self._active[torch.from_numpy(rows).to(self._active.device)] = 1 if active else 0
+
+    def make_filter(self, mask) -> DeviceFilter:
+        f = DeviceFilter(mask, self.device)
+        if f.n != self._n:
+            f.close()
+            raise ValueError("row_mask must have one byte per row")
+        return f
+
+    # --------------------------------------------------------------------- reads
+    def reconstruct(self, rows, dtype=None):
+        """The values that rows stand for.  Numpy positions: numpy float32, every position inside the index.  CUDA int64
+        positions: a CUDA tensor of ``dtype`` (default float32); a position outside the index -- an unfilled slot of a search -- gives zeros."""
+        on_device = _is_torch_cuda(rows)
+        if not on_device:
+            rows = np.ascontiguousarray(rows, dtype=np.int64).reshape(-1)
+            if rows.size and (rows.min() < 0 or rows.max() >= self._n):
+                raise ValueError("row position out of range")
+        at = self._positions(rows)
+        out = torch.empty((at.numel(), self.dim), dtype=torch.float32 if dtype is None or not on_device else dtype, device=self._dev)
+        kind = _type_of(out.dtype)
+        if at.numel():
+            check(lib.rag_mx4_read_device(self._st_ref, at.data_ptr(), at.numel(), out.data_ptr(), kind, self._kept.stream()))
+        return out if on_device else out.cpu().numpy()
+
+    # ------------------------------------------------------------------ products
+    def scores(self, q, begin: int = 0, end: Optional[int] = None):
+        """Every query against the rows [begin, end): float32 [nq, end - begin], a CUDA tensor for CUDA queries and numpy
+        for numpy ones."""
+        end = self._n if end is None else int(end)
+        begin = int(begin)
+        if not 0 <= begin <= end <= self._n:
+            raise ValueError("rows [begin, end) do not lie inside the index")
+        on_device = _is_torch_cuda(q)
+        q, ld = self._rows_in(q, "queries")
+        out = torch.empty((q.shape[0], end - begin), dtype=torch.float32, device=self._dev)
+        if out.numel():
+            check(lib.rag_mx4_scores_device(self._st_ref, begin, end, q.shape[0], q.data_ptr(), _type_of(q.dtype), ld,
+                                            self._normalize, out.data_ptr(), end - begin, self._kept.stream()))
+        return out if on_device else out.cpu().numpy()
+
+    def plan_groups(self, groups, nq: int, dtype=None) -> GroupPlan:
+        """Groups for ``scores_grouped`` that are used more than once: [n, 4] of (query begin, query end, row begin, row end),
+        for ``nq`` queries of ``dtype`` (default: float32).  Good as long as the index does not shrink."""
+        return GroupPlan(groups, nq, self._n, self.dim, torch.float32 if dtype is None else dtype, self.device)
+
+    def scores_grouped(self, q, groups):
+        """Ragged groups in one launch: the scores of each group, [its queries][its rows], one behind the other in a
+        flat float32 CUDA tensor.  ``groups``: a ``GroupPlan`` (whose ``split`` gives the views), or what ``plan_groups`` takes."""
+        q, ld = self._rows_in(q, "queries")
+        plan = groups if isinstance(groups, GroupPlan) else self.plan_groups(groups, q.shape[0], q.dtype)
+        if plan.device != self.device or plan.nq != q.shape[0] or plan.type != _type_of(q.dtype) or plan.n > self._n:
+            raise ValueError("the plan was made for other queries, another device or a longer index")
+        out = torch.empty((plan.total,), dtype=torch.float32, device=self._dev)
+        if plan.n_items:
+            plan._kept.stream()
+            check(lib.rag_mx4_scores_grouped_device(self._st_ref, q.shape[0], q.data_ptr(), plan.type, ld, self._normalize,
+                                                    plan.items.data_ptr(), plan.n_items, plan.widest, out.data_ptr(),
+                                                    self._kept.stream()))
+        return out
+
+    # -------------------------------------------------------------------- search
+    def search(self, q, k: int, min_score: Optional[float] = None, nprobe: int = 1, row_mask=None) -> Tuple[object, object]:
+        """``DeviceIndex.search`` over the stored rows: (D [nq, k] float32, I [nq, k] int64 row positions), best first, equal
+        scores by position, empty slots (-FLT_MAX, -1).  ``nprobe`` is accepted and unused."""
+        k = int(k)
+        if not 1 <= k <= MAX_K:
+            raise ValueError(f"k must be in [1, {MAX_K}]")
+        on_device = _is_torch_cuda(q)
+        dev = self._dev
+        if isinstance(row_mask, DeviceFilter) or _is_torch_cuda(row_mask):
+            m_ptr, keep = _device_mask_ptr(row_mask, self)
+        elif row_mask is not None:
+            m = np.ascontiguousarray(row_mask, dtype=np.uint8).reshape(-1)
+            if m.size != self._n:
+                raise ValueError("row_mask must have one byte per row")
+            keep = torch.from_numpy(m).to(dev)
+            m_ptr = keep.data_ptr()
+        else:
+            m_ptr = keep = None
+        q, ld = self._rows_in(q, "queries")
+        nq = q.shape[0]
+        D = torch.empty((nq, k), dtype=torch.float32, device=dev)
+        I = torch.empty((nq, k), dtype=torch.int64, device=dev)
+        if nq:
+            need = int(lib.rag_mx4_search_workspace(self._n, nq, k))
+            ws = torch.empty((need,), dtype=torch.uint8, device=dev)
+            check(lib.rag_mx4_search_device(self._st_ref, nq, q.data_ptr(), _type_of(q.dtype), ld, self._normalize, k,
+                                            -FLT_MAX if min_score is None else float(min_score), m_ptr,
+                                            None if self._active is None else self._active.data_ptr(), D.data_ptr(), I.data_ptr(),
+                                            ws.data_ptr(), need, self._kept.stream()))
+        self.last_path = "mx4" if self._n else "empty"
+        return (D, I) if on_device else (D.cpu().numpy(), I.cpu().numpy())
+
+    # --------------------------------------------------------------- persistence
+    def save(self, path: str) -> None:
+        """Rows as stored (the natural layout of ``packed``), soft deletes and metric, in one file."""
+        codes, scales = self.packed()
+        active = np.zeros(0, np.uint8) if self._active is None else self._active.cpu().numpy()
+        with open(path, "wb") as f:
+            np.savez(f, codes=codes.cpu().numpy(), scales=scales.cpu().numpy(), active=active, dim=np.int64(self.dim),
+                     cosine=np.int64(self._normalize))
+
+    @classmethod
+    def load(cls, path: str, device: int = 0) -> "QuantizedIndex":
+        with np.load(path, allow_pickle=False) as f:
+            self = cls.from_packed(f["codes"], f["scales"], int(f["dim"]), metric="cosine" if int(f["cosine"]) else "ip", device=device)
+            if f["active"].size:
+                self._active = torch.from_numpy(f["active"]).to(self._dev)
+                self._renew()
+        return self
+
+
+def _scale_places(groups: int) -> np.ndarray:
+    """Where the scale of every group lies inside a row's scale bytes (rag_hip.h, rag_mx4_layout)."""
+    g = np.arange(groups, dtype=np.int64)
+    return (g // 16) * 16 + (g % 4) * 4 + (g // 4) % 4
