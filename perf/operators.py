@@ -155,7 +155,7 @@ def prepare(case, seed):
         from rag_amd import QuantizedIndex
         state["index"] = QuantizedIndex.from_packed(codes, scales, dim, metric="ip")
         if op == "grouped" and case["shared"]:
-            state["plan"] = state["index"].plan_groups(state["groups"], state["q"].shape[0])   # the documents stay the same from question to question
+            state["plan"] = state["index"].plan_groups(state["groups"], state["q"].shape[0], dtype)   # the documents stay the same from question to question
     else:
         state["codes"], state["scales"] = codes, scales
     return state
