@@ -453,14 +453,15 @@ int rag_index_hybrid_mmr_batch_device(rag_index_t* h, int64_t nq, const float* q
  * Calls that write one store and calls that use it are ordered by the caller's streams. */
 enum rag_mx4_type { RAG_MX4_F32 = 0, RAG_MX4_BF16 = 1, RAG_MX4_F16 = 2 };
 typedef struct rag_mx4_store {
-    void* codes;      /* n * code_bytes, device memory on a 16-byte boundary; the layout inside a row is the library's own */
-    void* scales;     /* n * scale_bytes, likewise; zero bytes behind a row's groups */
+    void* codes;      /* device memory on a 16-byte boundary, code_bytes for every row, n rounded up to a multiple of 16 */
+    void* scales;     /* likewise, n * scale_bytes; zero bytes behind a row's groups */
     int64_t n;        /* rows, at most 2^31 - 1 */
     int32_t dim;      /* 1 .. 8192 */
     int32_t device;
 } rag_mx4_store_t;
-/* Bytes of one row.  Block b = i / 128 of a row holds element i at half-byte i % 128 of its 64 bytes; the scale of group
- * G = i / 32 is byte (G / 16) * 16 + (G % 4) * 4 + (G / 4) % 4.  Elements from dim to the end of the last block are zero. */
+/* Bytes of one row.  Its elements lie in blocks of 128: block b of row r is 64 bytes at (r / 16) * 16 * code_bytes + b * 1024 +
+ * (r % 16) * 64, element i in half-byte i % 128 (low half first), zeros behind dim.  The scale of group G = i / 32 is byte
+ * r * scale_bytes + (G / 16) * 16 + (G % 4) * 4 + (G / 4) % 4. */
 int rag_mx4_layout(int dim, int64_t* code_bytes, int64_t* scale_bytes);
 /* Quantise `count` rows of x_dev (elements of x_type, x_stride elements from row to row) as they are written:
  *   rows_dev NULL   to the rows [first, first + count)

@@ -6,13 +6,18 @@
 namespace rag {
 
 // A row of `dim` elements is padded with zeros to ks = ceil(dim / 128) blocks of 128 (what one matrix instruction takes
-// along the row).  codes: 64 bytes per block, element 2j of the row in the low half of byte j, 2j + 1 in the high half.
-// scales: one byte per group of 32; the bytes of four consecutive blocks lie together per group column, so that the lane
+// along the row): 64 bytes, element 2j in the low half of byte j, 2j + 1 in the high half.  codes: sixteen rows lie together,
+// block by block -- [row / 16][block][row % 16][64 bytes] -- so that one load of a wave (a block of sixteen rows) is one
+// contiguous KiB: 4M rows of 768 against one query 292 us with the rows one behind the other, 264 us like this.
+// scales: row after row, one byte per group of 32; the bytes of four consecutive blocks lie together per group column, so that the lane
 // that feeds group column g of a row fetches the scales of four blocks as one dword:
 //     group G of a row (block G / 4, column G % 4)  ->  byte (G / 16) * 16 + (G % 4) * 4 + (G / 4) % 4
 __host__ __device__ __forceinline__ int mx4_blocks(int dim) { return (dim + 127) / 128; }
 __host__ __device__ __forceinline__ int mx4_code_bytes(int dim) { return mx4_blocks(dim) * 64; }
 __host__ __device__ __forceinline__ int mx4_scale_bytes(int dim) { return (mx4_blocks(dim) + 3) / 4 * 16; }
+__host__ __device__ __forceinline__ size_t mx4_code_at(long long row, int code_ld, int block) {
+    return (size_t)(row >> 4) * 16 * code_ld + (size_t)block * 1024 + (row & 15) * 64;
+}
 __host__ __device__ __forceinline__ int mx4_scale_at(int group) { return (group >> 4) * 16 + (group & 3) * 4 + ((group >> 2) & 3); }
 
 constexpr int MX4_MAX_DIM = 8192;          // the query fragments of one matrix tile (2 KiB per block of 128) fit the LDS

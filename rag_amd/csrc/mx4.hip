@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
-        reinterpret_cast<unsigned*>(a.codes + (size_t)to * a.code_ld)[c] = bad ? 0u : w;
+        *reinterpret_cast<unsigned*>(a.codes + mx4_code_at(to, a.code_ld, c >> 4) + (c & 15) * 4) = bad ? 0u : w;
         if ((c & 3) == 0) a.scales[(size_t)to * a.scale_ld + mx4_scale_at(c >> 2)] = bad ? 255 : (uint8_t)(e + 127);
     }
 }
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(Mx4ReadArgs a) {
         const long long from = a.rows[i0 + r];
         float v[8] = {};
         if (from >= 0 && from < a.n) {
-            const unsigned w = reinterpret_cast<const unsigned*>(a.codes + (size_t)from * a.code_ld)[c];
+            const unsigned w = *reinterpret_cast<const unsigned*>(a.codes + mx4_code_at(from, a.code_ld, c >> 4) + (c & 15) * 4);
             const unsigned b = a.scales[(size_t)from * a.scale_ld + mx4_scale_at(c >> 2)];
             const float f = b == 255 ? NAN : b == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(b << 23);
             v2f p;
@@ -370,36 +370,41 @@ __device__ __forceinline__ float columns_sum(float v0, float v1, float v2, float
     return swap_add16(swap_add32(v0, v2), swap_add32(v1, v3));
 }
 
-// ND digits, MT tiles of queries, NB blocks of 16 rows per wave, U row blocks of 128 fetched together, NW waves.
+// ND digits, MT tiles of queries, NB blocks of 16 rows per wave, U blocks of 128 along the row fetched together, NW waves;
+// ONE: U blocks are the whole row.
 //
 // A wave takes 16 NB rows at a time and keeps the next U blocks of them in flight while the present ones go through the
-// matrix unit; nothing but the query fragments goes through LDS, and there is no barrier after they are staged.
-template <int ND, int MT, int NB, int U, int NW>
+// matrix unit; nothing but the query fragments goes through LDS, and there is no barrier after they are staged.  The fetch
+// ahead is unconditional (past the last rows it repeats them): behind a branch the compiler would wait for it at once.
+template <int ND, int MT, int NB, int U, int NW, bool ONE, bool NT>
 __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     constexpr int QPT = Mx4Digits<ND>::QPT;
     constexpr int QB = MT * QPT;
     constexpr int SW = (U + 3) / 4;                             // scale dwords per fetch
+    const int ks = ONE ? U : a.ks, ksu = ONE ? U : a.ksu;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     uint8_t* frag = smem;
-    uint8_t* sc = frag + (size_t)a.ksu * MT * 2048;
-    float* inv = reinterpret_cast<float*>(sc + (size_t)((a.ksu + 3) / 4) * MT * 256);
+    uint8_t* sc = frag + (size_t)ksu * MT * 2048;
+    float* inv = reinterpret_cast<float*>(sc + (size_t)((ksu + 3) / 4) * MT * 256);
 
+    // rows [row0, row0 + rows) against queries [q0, q0 + nqh); this wave takes the tiles of 16 NB rows first, first + stride, ...
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     long long row0, at, ld;
-    int rows, q0, nqh;
+    int rows, q0, nqh, first = wave, stride = NW;
     if (a.items) {
         const Mx4Item it = a.items[blockIdx.x];
         row0 = it.row0; at = it.at; ld = it.ld; rows = it.rows; q0 = it.q0; nqh = it.nq;
+    } else if (a.nqb == 1) {
+        row0 = a.row0; at = 0; ld = a.out_ld; rows = (int)a.rows; q0 = 0; nqh = a.nq;
+        first = (int)blockIdx.x * NW + wave;
+        stride = (int)gridDim.x * NW;
     } else {
         // consecutive workgroups go to the eight dies in turn: the query blocks of a slab stay on one die, whose L2 then
         // holds the slab's rows for all of them
         const long long b = blockIdx.x;
-        long long s = b;
-        int qb = 0;
-        if (a.nqb > 1) {
-            const long long i = b >> 3;
-            s = (i / a.nqb) * 8 + (b & 7);
-            qb = (int)(i % a.nqb);
-        }
+        const long long i = b >> 3;
+        const long long s = (i / a.nqb) * 8 + (b & 7);
+        const int qb = (int)(i % a.nqb);
         const long long lo = s * a.slab;
         if (lo >= a.rows) return;
         rows = (int)(a.rows - lo < a.slab ? a.rows - lo : a.slab);
@@ -409,36 +414,38 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         at = (long long)q0 * a.out_ld + lo;
         ld = a.out_ld;
     }
-    mx4_stage_queries<ND, MT, NW * 64>(a, q0, nqh, frag, sc, inv);
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n16 = lane & 15, col = lane >> 4;
-    const int tiles = (rows + 16 * NB - 1) / (16 * NB);
-    if (wave >= tiles) return;
-    const int sd = (a.ks + 3) / 4;                              // scale dwords of a lane per row
+    const int tiles = rows / (16 * NB) + (rows % (16 * NB) != 0);
+    const int sd = (ks + 3) / 4;                                // scale dwords of a lane per row
+    float* out = a.out + at;
 
     struct Buf {
         v4i w[NB][U];
         int s[NB][SW];
     };
     auto load = [&](Buf& b, int tile, int ks0) {
+        const int base = tile * (16 * NB), last = rows - 1 - base;
+        const long long r0 = row0 + base;                       // uniform over the wave; what differs between lanes fits 32 bits
+        const uint8_t* wbase = a.codes + (r0 >> 4) * 16 * a.code_ld + col * 16;
+        const uint8_t* sbase = a.scales + r0 * a.scale_ld + col * 4;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            int r = tile * 16 * NB + nb * 16 + n16;
-            r = r < rows ? r : rows - 1;                        // rows past the end: fetched again, never stored
-            const uint8_t* w = a.codes + (size_t)(row0 + r) * a.code_ld + col * 16;
-            const uint8_t* s = a.scales + (size_t)(row0 + r) * a.scale_ld + col * 4;
+            int r = nb * 16 + n16;
+            r = r < last ? r : last;                            // rows past the end: fetched again, never stored
+            const int l = r + (int)(r0 & 15);
+            const unsigned wo = __umul24(l >> 4, 16 * a.code_ld) + (l & 15) * 64;
+            const unsigned so = __umul24(r, a.scale_ld);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int k = ks0 + u < a.ks ? ks0 + u : a.ks - 1;      // blocks past the row's meet zero digits
-                b.w[nb][u] = *reinterpret_cast<const v4i*>(w + k * 64);
+                const int k = ONE ? u : ks0 + u < ks ? ks0 + u : ks - 1;      // blocks past the row's meet zero digits
+                const v4i* w = reinterpret_cast<const v4i*>(wbase + wo + k * 1024);
+                b.w[nb][u] = NT ? __builtin_nontemporal_load(w) : *w;
             }
 #pragma unroll
             for (int d = 0; d < SW; ++d) {
-                const int k = (ks0 >> 2) + d < sd ? (ks0 >> 2) + d : sd - 1;
-                b.s[nb][d] = *reinterpret_cast<const int*>(s + k * 16);
+                const int k = ONE ? d : (ks0 >> 2) + d < sd ? (ks0 >> 2) + d : sd - 1;
+                b.s[nb][d] = *reinterpret_cast<const int*>(sbase + so + k * 16);
             }
-            if constexpr (U < 4) b.s[nb][0] = (int)((unsigned)b.s[nb][0] >> ((ks0 & 3) * 8));
         }
     };
     v4f acc[MT][NB];
@@ -449,19 +456,24 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
             for (int nb = 0; nb < NB; ++nb) acc[mt][nb] = (v4f){0.f, 0.f, 0.f, 0.f};
     };
     auto multiply = [&](const Buf& b, int ks0) {
+        int fl = lane;
+        if constexpr (MT > 1) asm volatile("" : "+v"(fl));      // more than one tile's fragments do not fit the registers: read from LDS each time
         static_for<U>([&](auto uc) {
             constexpr int u = decltype(uc)::value;
+            constexpr bool SHIFT = !ONE && U < 4;               // the fetch may begin inside a scale dword
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const v4i* f = reinterpret_cast<const v4i*>(frag + (size_t)((ks0 + u) * MT + mt) * 2048) + lane;
+                const v4i* f = reinterpret_cast<const v4i*>(frag + (size_t)((ks0 + u) * MT + mt) * 2048) + fl;
                 const v4i lo = f[0], hi = f[64];
                 const v8i x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                int xs = reinterpret_cast<const int*>(sc + (size_t)(((ks0 + (U < 4 ? 0 : u)) >> 2) * MT + mt) * 256)[lane];
-                if constexpr (U < 4) xs = (int)((unsigned)xs >> ((ks0 & 3) * 8));
+                int xs = reinterpret_cast<const int*>(sc + (size_t)(((ks0 + (SHIFT ? 0 : u)) >> 2) * MT + mt) * 256)[fl];
+                if constexpr (SHIFT) xs = (int)((unsigned)xs >> ((ks0 & 3) * 8));
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     const v8i y = __builtin_shufflevector(b.w[nb][u], b.w[nb][u], 0, 1, 2, 3, -1, -1, -1, -1);
-                    acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, acc[mt][nb], 0, 4, u & 3, xs, u & 3, b.s[nb][u / 4]);
+                    int ys = b.s[nb][u / 4];
+                    if constexpr (SHIFT) ys = (int)((unsigned)ys >> ((ks0 & 3) * 8));
+                    acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, acc[mt][nb], 0, 4, u & 3, xs, u & 3, ys);
                 }
             }
         });
@@ -477,37 +489,55 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
                 const int r = (tile * NB + nb) * 16 + n16, s = mt * QPT + col;
                 float y = columns_sum(v[0], v[1], v[2], ND == 5 ? 0.f : v[3]);
                 if (ND == 5) y += v[3];
-                if (col < QPT && s < nqh && r < rows) a.out[at + (long long)s * ld + r] = y * inv[s];
+                if (col < QPT && s < nqh && r < rows) out[(long long)s * ld + r] = y * inv[s];
             }
         }
     };
 
     Buf x, y;
-    int t = wave, k = 0;
-    load(x, t, 0);
+    int t = first, k = 0;
+    load(x, t < tiles ? t : tiles - 1, 0);                      // on its way while the queries are split
+    mx4_stage_queries<ND, MT, NW * 64>(a, q0, nqh, frag, sc, inv);
+    if (first >= tiles) return;
     clear();
-    auto step = [&](Buf& now, Buf& next) -> bool {              // false: that was the last one
-        int t2 = t, k2 = k + U;
-        if (k2 >= a.ksu) { k2 = 0; t2 += NW; }
-        if (t2 < tiles) load(next, t2, k2);
-        multiply(now, k);
+    for (;;) {
+        // where the piece behind this one lies, and the one behind that
+        auto next = [&](int& t2, int& k2) {
+            if (!ONE) {
+                k2 += U;
+                if (k2 < ksu) return;
+                k2 = 0;
+            }
+            t2 += stride;
+        };
+        int t2 = t, k2 = k;
+        next(t2, k2);
+        load(y, t2 < tiles ? t2 : tiles - 1, k2);
+        __builtin_amdgcn_sched_barrier(0);                      // the fetch goes out before the products wait for theirs
+        multiply(x, k);
         if (k2 == 0) {
             store(t);
             clear();
         }
+        if (t2 >= tiles) break;
         t = t2;
         k = k2;
-        return t2 < tiles;
-    };
-    for (;;) {
-        if (!step(x, y)) break;
-        if (!step(y, x)) break;
+        next(t, k);
+        load(x, t < tiles ? t : tiles - 1, k);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(y, k2);
+        if (k == 0) {
+            store(t2);
+            clear();
+        }
+        if (t >= tiles) break;
     }
 }
 
 // Which kernel a product takes: from the queries that meet a row, and the row's length.
 struct Mx4Shape {
     int nd, mt, nb, u, nw, ksu, qb;
+    bool one, nt;
     size_t lds;
 };
 static size_t mx4_lds(int ks, int u, int mt) {
@@ -521,13 +551,14 @@ static Mx4Shape mx4_shape(int type, int dim, long long nq) {
     const int qpt = p.nd == 5 ? 3 : 4;
     const long long need = (nq + qpt - 1) / qpt;
     auto fetch = [&](int mt) {
-        if (mt <= 2) return ks <= 4 ? ks : ks <= 6 ? 6 : ks <= 8 || (ks & 7) == 0 || (ks & 7) > 4 ? 8 : 4;
-        if (mt == 4) return ks <= 4 ? ks : ks == 6 ? 6 : (ks & 3) == 0 ? 4 : (ks & 1) == 0 ? 2 : 1;
-        return ks <= 4 ? ks : (ks & 3) == 0 ? 4 : (ks & 1) == 0 ? 2 : 1;
+        if (mt <= 2) return ks <= 8 ? ks : (ks & 7) == 0 || (ks & 7) > 4 ? 8 : 4;
+        if (mt == 4) return ks <= 4 ? ks : (ks & 3) == 0 ? 4 : (ks & 1) == 0 ? 2 : 1;
+        return (ks & 1) == 0 ? 2 : 1;
     };
     p.mt = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8;
     while (p.mt > 1 && mx4_lds(ks, fetch(p.mt), p.mt) > 160 * 1024) p.mt /= 2;
     p.u = fetch(p.mt);
+    p.one = p.u == ks;
     p.nb = p.mt <= 2 ? 1 : 2;
     p.nw = p.mt == 8 ? 8 : 4;
     p.ksu = (ks + p.u - 1) / p.u * p.u;
@@ -536,10 +567,10 @@ static Mx4Shape mx4_shape(int type, int dim, long long nq) {
     return p;
 }
 
-template <int ND, int MT, int NB, int U, int NW>
+template <int ND, int MT, int NB, int U, int NW, bool ONE, bool NT>
 static int mx4_launch(const Mx4ScoreArgs& a, long long grid, size_t lds, int device, hipStream_t s) {
     static bool attr_set[64] = {};          // per device: the attribute belongs to the device's code object
-    auto kern = mx4_scores_kernel<ND, MT, NB, U, NW>;
+    auto kern = mx4_scores_kernel<ND, MT, NB, U, NW, ONE, NT>;
     if (lds > 48 * 1024 && !attr_set[device & 63]) {
         RAG_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         attr_set[device & 63] = true;
@@ -550,11 +581,17 @@ static int mx4_launch(const Mx4ScoreArgs& a, long long grid, size_t lds, int dev
 }
 template <int ND>
 static int mx4_launch_nd(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s) {
-#define MX4_CASE(MT, NB, U, NW) if (p.mt == MT && p.u == U) return mx4_launch<ND, MT, NB, U, NW>(a, grid, p.lds, device, s)
-    MX4_CASE(1, 1, 1, 4); MX4_CASE(1, 1, 2, 4); MX4_CASE(1, 1, 3, 4); MX4_CASE(1, 1, 4, 4); MX4_CASE(1, 1, 6, 4); MX4_CASE(1, 1, 8, 4);
-    MX4_CASE(2, 1, 1, 4); MX4_CASE(2, 1, 2, 4); MX4_CASE(2, 1, 3, 4); MX4_CASE(2, 1, 4, 4); MX4_CASE(2, 1, 6, 4); MX4_CASE(2, 1, 8, 4);
-    MX4_CASE(4, 2, 1, 4); MX4_CASE(4, 2, 2, 4); MX4_CASE(4, 2, 3, 4); MX4_CASE(4, 2, 4, 4); MX4_CASE(4, 2, 6, 4);
-    MX4_CASE(8, 2, 1, 8); MX4_CASE(8, 2, 2, 8); MX4_CASE(8, 2, 3, 8); MX4_CASE(8, 2, 4, 8);
+#define MX4_CASE(MT, NB, U, NW, ONE) if (p.mt == MT && p.u == U && p.one == ONE) return p.nt ? mx4_launch<ND, MT, NB, U, NW, ONE, true>(a, grid, p.lds, device, s) : mx4_launch<ND, MT, NB, U, NW, ONE, false>(a, grid, p.lds, device, s)
+#define MX4_FEW(MT) \
+    MX4_CASE(MT, 1, 1, 4, true); MX4_CASE(MT, 1, 2, 4, true); MX4_CASE(MT, 1, 3, 4, true); MX4_CASE(MT, 1, 4, 4, true); \
+    MX4_CASE(MT, 1, 5, 4, true); MX4_CASE(MT, 1, 6, 4, true); MX4_CASE(MT, 1, 7, 4, true); MX4_CASE(MT, 1, 8, 4, true); \
+    MX4_CASE(MT, 1, 4, 4, false); MX4_CASE(MT, 1, 8, 4, false)
+    MX4_FEW(1);
+    MX4_FEW(2);
+    MX4_CASE(4, 2, 1, 4, true); MX4_CASE(4, 2, 2, 4, true); MX4_CASE(4, 2, 3, 4, true); MX4_CASE(4, 2, 4, 4, true);
+    MX4_CASE(4, 2, 1, 4, false); MX4_CASE(4, 2, 2, 4, false); MX4_CASE(4, 2, 4, 4, false);
+    MX4_CASE(8, 2, 1, 8, true); MX4_CASE(8, 2, 2, 8, true); MX4_CASE(8, 2, 1, 8, false); MX4_CASE(8, 2, 2, 8, false);
+#undef MX4_FEW
 #undef MX4_CASE
     return fail(RAG_ERR_INVALID, "internal: no four-bit product kernel for this shape");
 }
@@ -601,8 +638,9 @@ static Mx4ScoreArgs mx4_score_args(const rag_mx4_store_t* st, const Mx4Shape& p,
 // scores of rows [row0, row0 + rows) (checked by the caller)
 static int mx4_scores(const rag_mx4_store_t* st, long long row0, long long rows, long long nq, const void* q, int q_type, long long ldq,
                       int normalize, float* out, long long out_ld, hipStream_t s) {
-    const Mx4Shape p = mx4_shape(q_type, st->dim, nq);
+    Mx4Shape p = mx4_shape(q_type, st->dim, nq);
     Mx4ScoreArgs a = mx4_score_args(st, p, q, q_type, ldq, normalize, out);
+    p.nt = nq <= p.qb && rows * a.code_ld > (getenv("MXNT") ? atoll(getenv("MXNT")) << 20 : 64LL << 20);
     a.row0 = row0;
     a.rows = rows;
     a.out_ld = out_ld;
@@ -610,12 +648,11 @@ static int mx4_scores(const rag_mx4_store_t* st, long long row0, long long rows,
     a.nqb = (int)((nq + p.qb - 1) / p.qb);
     const long long unit = 16LL * p.nb * p.nw;                  // rows of one step of a workgroup
     const long long units = (rows + unit - 1) / unit;
-    const long long want = std::max<long long>(1, (p.mt == 8 ? 2048 : 1024) / a.nqb);     // slabs
+    if (a.nqb == 1) return mx4_launch_any(p, a, std::min<long long>(units, getenv("MXG") ? atoi(getenv("MXG")) : p.mt == 8 ? 256 : p.mt == 4 ? 512 : 1024), st->device, s);
+    const long long want = std::max<long long>(1, 2048 / a.nqb);                          // slabs
     a.slab = (units + want - 1) / want * unit;
-    a.slab = std::min<long long>(a.slab, 1LL << 30);
     const long long slabs = (rows + a.slab - 1) / a.slab;
-    const long long grid = a.nqb > 1 ? (slabs + 7) / 8 * 8 * a.nqb : slabs;
-    return mx4_launch_any(p, a, grid, st->device, s);
+    return mx4_launch_any(p, a, (slabs + 7) / 8 * 8 * a.nqb, st->device, s);
 }
 
 int direct_select_segments(long long nq, long long n_row, long long seg_rows, int k, float min_score, const uint8_t* mask,

@@ -139,13 +139,15 @@ class QuantizedIndex:
         have = 0 if self._codes is None else self._codes.shape[0]
         if nrows <= have:
             return
+        nrows = (nrows + 15) // 16 * 16                      # sixteen rows lie together
         dev = self._dev
         made = _Kept(self.device)
         codes = torch.zeros((nrows, self._code_bytes), dtype=torch.uint8, device=dev)
         scales = torch.zeros((nrows, self._scale_bytes), dtype=torch.uint8, device=dev)
         owner = torch.zeros((nrows,), dtype=torch.int32, device=dev)
         if self._n:
-            codes[:self._n] = self._codes[:self._n]
+            used = (self._n + 15) // 16 * 16
+            codes[:used] = self._codes[:used]
             scales[:self._n] = self._scales[:self._n]
         self._codes, self._scales, self._owner, self._kept = codes, scales, owner, made
         self._renew()
@@ -229,12 +231,14 @@ class QuantizedIndex:
         self = cls(dim, metric=metric, device=device, capacity=n)
         if n:
             dev = self._dev
-            self._codes[:, :16 * groups] = codes.to(dev)
+            rows = torch.zeros((self._codes.shape[0], self._code_bytes), dtype=torch.uint8, device=dev)
+            rows[:n, :16 * groups] = codes.to(dev)
             if self.dim % 32:
-                self._codes[:, (self.dim + 1) // 2:] = 0
+                rows[:, (self.dim + 1) // 2:] = 0
                 if self.dim % 2:
-                    self._codes[:, self.dim // 2] &= 15
-            self._scales[:, torch.from_numpy(_scale_places(groups)).to(dev)] = scales.to(dev)
+                    rows[:, self.dim // 2] &= 15
+            self._codes.view(-1, self._code_bytes // 64, 16, 64).copy_(rows.view(-1, 16, self._code_bytes // 64, 64).transpose(1, 2))
+            self._scales[:n, torch.from_numpy(_scale_places(groups)).to(dev)] = scales.to(dev)
             self._n = n
             self._renew()
         return self
@@ -246,7 +250,9 @@ class QuantizedIndex:
             dev = self._dev
             return (torch.empty((0, 16 * groups), dtype=torch.uint8, device=dev), torch.empty((0, groups), dtype=torch.uint8, device=dev))
         places = torch.from_numpy(_scale_places(groups)).to(self._codes.device)
-        return self._codes[:self._n, :16 * groups].clone(), self._scales[:self._n][:, places]
+        used = (self._n + 15) // 16 * 16
+        rows = self._codes[:used].view(-1, self._code_bytes // 64, 16, 64).transpose(1, 2).reshape(used, self._code_bytes)
+        return rows[:self._n, :16 * groups].contiguous(), self._scales[:self._n][:, places]
 
     def set_active(self, rows, active: bool) -> None:
         """Hide rows from every search, or show them again (vector_db/qdrant_client.py:826-883)."""
