@@ -276,11 +276,12 @@ struct Mx4ScoreArgs {
     const void* q;
     long long ldq;               // elements
     int q_type, q_vec, dim, ks, ksu, code_ld, scale_ld, normalize;
+    size_t code_bytes, scale_bytes;      // of the whole store
     float* out;
     // grouped: one workgroup per item
     const Mx4Item* items;
     // dense: rows [row0, row0 + rows) cut into slabs, every slab against blocks of QB queries
-    long long row0, rows, slab, out_ld;
+    long long row0, rows, slab, slabs, out_ld;
     int nq, nqb;
 };
 
@@ -289,23 +290,34 @@ struct Mx4ScoreArgs {
 // elements 64 + 16 c ..; scale of lane l (either operand): elements 32 c .. 32 c + 31.  Result register r of lane l:
 // (eight-bit row 4 c + r, four-bit row l % 16).
 //
-// Digit j < 4 of query s of a tile is eight-bit row 4 j + s (result register s, column j); the fifth digit is row 4 s + 3
-// (register 3, column s).
-template <int ND>
+// Digit j < 4 of query s of a tile is eight-bit row 4 s + j: the four registers of column s, added without leaving the lane.
+// Fifth digits (fp32): up to three queries share their tile with them -- rows 12 + s: register s of column 3, fetched from
+// there by fifth_digits().  More queries put four to a tile and have the fifth digits of each four tiles in one more tile, query s
+// of tile t in row 4 s + t: register t of column s, where they are wanted.
+template <int ND, int MT>
 struct Mx4Digits {
-    static constexpr int QPT = ND == 5 ? 3 : 4;        // queries per tile of 16 eight-bit rows
-    static __device__ __forceinline__ int row(int digit, int s) { return digit < 4 ? 4 * digit + s : 4 * s + 3; }
+    static constexpr bool INSIDE = ND == 5 && MT == 1;           // fifth digits in the tile itself
+    static constexpr int EX = ND == 5 && !INSIDE ? (MT + 3) / 4 : 0;
+    static constexpr int TILES = MT + EX;
+    static constexpr int QPT = INSIDE ? 3 : 4;                   // queries per tile of 16 eight-bit rows
 };
 
-// queries [q0, q0 + nqh) -> digit fragments in LDS.  frag[(block * MT + tile) * 2 + half][lane][16 bytes], then the scales
-// sc[(block / 4) * MT + tile][lane][block % 4], then 1 / |q|.  Blocks past the row's are zero.
+// queries [q0, q0 + nqh) -> digit fragments in LDS.  frag[(block * TILES + tile) * 2 + half][lane][16 bytes], then the scales
+// sc[(block / 4) * TILES + tile][lane][block % 4], then 1 / |q|.  Blocks past the row's are zero: they meet a real block of the
+// row again.  What the fragments of absent queries hold does not matter: it stays in result rows that nobody reads.
 template <int ND, int MT, int NT>
 __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long long q0, int nqh, uint8_t* frag, uint8_t* sc, float* inv) {
-    constexpr int QPT = Mx4Digits<ND>::QPT;
+    typedef Mx4Digits<ND, MT> L;
+    constexpr int QPT = L::QPT, TILES = L::TILES;
     const int tid = threadIdx.x;
-    const v4i zero = {0, 0, 0, 0};
-    const int words = (a.ksu * MT * 2048 + (a.ksu + 3) / 4 * MT * 256) / 16;          // frag and sc are adjacent
-    for (int i = tid; i < words; i += NT) reinterpret_cast<v4i*>(frag)[i] = zero;
+    if (a.ksu > a.ks) {
+        const v4i zero = {0, 0, 0, 0};
+        v4i* f = reinterpret_cast<v4i*>(frag + (size_t)a.ks * TILES * 2048);
+        for (int i = tid; i < (a.ksu - a.ks) * TILES * 128; i += NT) f[i] = zero;
+        v4i* s = reinterpret_cast<v4i*>(sc + (size_t)(a.ks / 4) * TILES * 256);
+        for (int i = tid; i < ((a.ksu + 3) / 4 - a.ks / 4) * TILES * 16; i += NT) s[i] = zero;
+        __syncthreads();
+    }
     const size_t esize = a.q_type == RAG_MX4_F32 ? 4 : 2;
     const char* q = static_cast<const char*>(a.q) + (size_t)q0 * a.ldq * esize;
     for (int s = tid >> 6; s < MT * QPT; s += NT / 64) {
@@ -313,7 +325,6 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long lo
         if (a.normalize && s < nqh) f = wave_inv_norm(q + (size_t)s * a.ldq * esize, a.q_type, a.dim, tid & 63);
         if ((tid & 63) == 0) inv[s] = f;
     }
-    __syncthreads();
     const int upq = a.ks * 32;                                  // units of 4 elements per query
     for (int u = tid; u < nqh * upq; u += NT) {
         const int s = u / upq, c = u - s * upq;
@@ -334,8 +345,8 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long lo
         const int block = c >> 5, in = c & 31;                  // 4 elements `in` of the block
         const int col = (in >> 2) & 3, half = in >> 4;
         const int tile = s / QPT, slot = s - tile * QPT;
-        uint8_t* to = frag + (size_t)((block * MT + tile) * 2 + half) * 1024 + col * 256 + (in & 3) * 4;
-        uint8_t* ts = sc + (size_t)((block >> 2) * MT + tile) * 256 + (in >> 3) * 64 + (block & 3);
+        uint8_t* to = frag + (size_t)(block * TILES * 2 + half) * 1024 + col * 256 + (in & 3) * 4;
+        uint8_t* ts = sc + (size_t)((block >> 2) * TILES) * 256 + (in >> 3) * 64 + (block & 3);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] *= down;
 #pragma unroll
@@ -349,25 +360,22 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long lo
             int p = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], 0, false);
             p = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], p, true);
             if (bad) p = d == 0 ? 0x7f7f7f7f : 0;               // NaN: every score of the query is NaN
-            const int m = Mx4Digits<ND>::row(d, slot);
-            *reinterpret_cast<int*>(to + m * 16) = p;
-            if ((in & 7) == 0) ts[m * 4] = (uint8_t)(127 + e - 5 * d);
+            const int m = d < 4 ? 4 * slot + d : L::INSIDE ? 12 + slot : 4 * slot + (tile & 3);
+            const int at = d < 4 || L::INSIDE ? tile : MT + (tile >> 2);
+            *reinterpret_cast<int*>(to + at * 2048 + m * 16) = p;
+            if ((in & 7) == 0) ts[at * 256 + m * 4] = (uint8_t)(127 + e - 5 * d);
         }
     }
     __syncthreads();
 }
 
-__device__ __forceinline__ float swap_add32(float a, float b) {      // lanes 0..31: a's two halves added; 32..63: b's
-    const v2u r = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false));
-    return __uint_as_float(r.x) + __uint_as_float(r.y);
-}
-__device__ __forceinline__ float swap_add16(float a, float b) {      // even columns of 16 lanes: a's pair added; odd: b's
-    const v2u r = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false));
-    return __uint_as_float(r.x) + __uint_as_float(r.y);
-}
-// four values, each to be summed over the four columns of lanes: column c is left with the sum of v_c
-__device__ __forceinline__ float columns_sum(float v0, float v1, float v2, float v3) {
-    return swap_add16(swap_add32(v0, v2), swap_add32(v1, v3));
+// lanes of column s (0, 1, 2) receive v_s of column 3
+__device__ __forceinline__ float fifth_digits(float v0, float v1, float v2) {
+    const v2u a = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(v0), __float_as_uint(v2), false, false));
+    const v2u b = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(v1), __float_as_uint(v1), false, false));
+    // a.y: columns 2, 3 of v0, then 2, 3 of v2; b.y: columns 2, 3 of v1, twice
+    const v2u r = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false));
+    return __uint_as_float(r.y);                                // the odd columns of both in turn: v0, v1, v2, v1 of column 3
 }
 
 // ND digits, MT tiles of queries, NB blocks of 16 rows per wave, U blocks of 128 along the row fetched together, NW waves;
@@ -378,14 +386,14 @@ __device__ __forceinline__ float columns_sum(float v0, float v1, float v2, float
 // ahead is unconditional (past the last rows it repeats them): behind a branch the compiler would wait for it at once.
 template <int ND, int MT, int NB, int U, int NW, bool ONE, bool NT>
 __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
-    constexpr int QPT = Mx4Digits<ND>::QPT;
-    constexpr int QB = MT * QPT;
+    typedef Mx4Digits<ND, MT> L;
+    constexpr int QPT = L::QPT, TILES = L::TILES, QB = MT * QPT;
     constexpr int SW = (U + 3) / 4;                             // scale dwords per fetch
     const int ks = ONE ? U : a.ks, ksu = ONE ? U : a.ksu;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     uint8_t* frag = smem;
-    uint8_t* sc = frag + (size_t)ksu * MT * 2048;
-    float* inv = reinterpret_cast<float*>(sc + (size_t)((ksu + 3) / 4) * MT * 256);
+    uint8_t* sc = frag + (size_t)ksu * TILES * 2048;
+    float* inv = reinterpret_cast<float*>(sc + (size_t)((ksu + 3) / 4) * TILES * 256);
 
     // rows [row0, row0 + rows) against queries [q0, q0 + nqh); this wave takes the tiles of 16 NB rows first, first + stride, ...
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -399,14 +407,13 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         first = (int)blockIdx.x * NW + wave;
         stride = (int)gridDim.x * NW;
     } else {
-        // consecutive workgroups go to the eight dies in turn: the query blocks of a slab stay on one die, whose L2 then
-        // holds the slab's rows for all of them
-        const long long b = blockIdx.x;
-        const long long i = b >> 3;
-        const long long s = (i / a.nqb) * 8 + (b & 7);
-        const int qb = (int)(i % a.nqb);
+        // workgroups go to the eight dies in turn: each die takes a contiguous part of the (slab, query block) pairs, so the
+        // query blocks of a slab stay on one die, whose L2 then holds the slab's rows for all of them
+        const long long pairs = a.slabs * a.nqb, id = (blockIdx.x & 7) * ((pairs + 7) >> 3) + (blockIdx.x >> 3);
+        if (id >= pairs || (blockIdx.x >> 3) >= (pairs + 7) >> 3) return;
+        const long long s = id / a.nqb;
+        const int qb = (int)(id % a.nqb);
         const long long lo = s * a.slab;
-        if (lo >= a.rows) return;
         rows = (int)(a.rows - lo < a.slab ? a.rows - lo : a.slab);
         q0 = qb * QB;
         nqh = a.nq - q0 < QB ? a.nq - q0 : QB;
@@ -423,73 +430,91 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         v4i w[NB][U];
         int s[NB][SW];
     };
+    // Rows are fetched through buffer descriptors that end with the store: rows past the last one of a piece are fetched and
+    // never stored, what would lie behind the store comes back as zeros.  (The check is lane offset >= size - uniform offset: the
+    // uniform part, a block or scale dword of the tile's first row, always lies inside the store.)
+    const int l0 = (int)(row0 & 15) + n16;                      // tiles start at multiples of 16 from row0
+    const int wo = (l0 >> 4) * 16 * a.code_ld + (l0 & 15) * 64 + col * 16, so = n16 * a.scale_ld + col * 4;
+    constexpr int AUX = NT ? 2 : 0;                             // 2: not to be kept in the caches
     auto load = [&](Buf& b, int tile, int ks0) {
-        const int base = tile * (16 * NB), last = rows - 1 - base;
-        const long long r0 = row0 + base;                       // uniform over the wave; what differs between lanes fits 32 bits
-        const uint8_t* wbase = a.codes + (r0 >> 4) * 16 * a.code_ld + col * 16;
-        const uint8_t* sbase = a.scales + r0 * a.scale_ld + col * 4;
+        const long long r0 = row0 + (long long)tile * (16 * NB);
+        const size_t wat = (size_t)(r0 >> 4) * 16 * a.code_ld, sat = (size_t)r0 * a.scale_ld;
+        const size_t wleft = a.code_bytes - wat, sleft = a.scale_bytes - sat;
+        const auto wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.codes) + wat, 0, (int)(wleft < 0x7fffffffu ? wleft : 0x7fffffffu), 0x00027000);
+        const auto sr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.scales) + sat, 0, (int)(sleft < 0x7fffffffu ? sleft : 0x7fffffffu), 0x00027000);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            int r = nb * 16 + n16;
-            r = r < last ? r : last;                            // rows past the end: fetched again, never stored
-            const int l = r + (int)(r0 & 15);
-            const unsigned wo = __umul24(l >> 4, 16 * a.code_ld) + (l & 15) * 64;
-            const unsigned so = __umul24(r, a.scale_ld);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int k = ONE ? u : ks0 + u < ks ? ks0 + u : ks - 1;      // blocks past the row's meet zero digits
-                const v4i* w = reinterpret_cast<const v4i*>(wbase + wo + k * 1024);
-                b.w[nb][u] = NT ? __builtin_nontemporal_load(w) : *w;
+                b.w[nb][u] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(wr, wo + nb * 16 * a.code_ld, k * 1024, AUX));
             }
 #pragma unroll
             for (int d = 0; d < SW; ++d) {
                 const int k = ONE ? d : (ks0 >> 2) + d < sd ? (ks0 >> 2) + d : sd - 1;
-                b.s[nb][d] = *reinterpret_cast<const int*>(sbase + so + k * 16);
+                b.s[nb][d] = (int)__builtin_amdgcn_raw_buffer_load_b32(sr, so + nb * 16 * a.scale_ld, k * 16, 0);
             }
         }
     };
-    v4f acc[MT][NB];
-    auto clear = [&]() {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) acc[mt][nb] = (v4f){0.f, 0.f, 0.f, 0.f};
-    };
-    auto multiply = [&](const Buf& b, int ks0) {
+    v4f acc[TILES][NB];
+    auto multiply = [&](const Buf& b, int ks0, auto first_of_row) {
+        constexpr bool FIRST = decltype(first_of_row)::value;   // begins the sums at zero
+        constexpr bool SHIFT = !ONE && U < 4;                   // the fetch may begin inside a scale dword
+        const uint8_t* f = frag + (size_t)ks0 * TILES * 2048;
         int fl = lane;
-        if constexpr (MT > 1) asm volatile("" : "+v"(fl));      // more than one tile's fragments do not fit the registers: read from LDS each time
-        static_for<U>([&](auto uc) {
-            constexpr int u = decltype(uc)::value;
-            constexpr bool SHIFT = !ONE && U < 4;               // the fetch may begin inside a scale dword
+        if constexpr (TILES > 1) asm volatile("" : "+v"(fl));      // more than one tile's fragments do not fit the registers: read from LDS each time
+        // query fragments one tile ahead: the LDS latency passes under the products of the tile before
+        v4i lo[2], hi[2];
+        int xs[2];
+        auto fetch = [&](auto ic) {
+            constexpr int i = decltype(ic)::value, u = i / TILES, mt = i % TILES;
+            const v4i* p = reinterpret_cast<const v4i*>(f + i * 2048) + fl;
+            lo[i & 1] = p[0];
+            hi[i & 1] = p[64];
+            const int x = reinterpret_cast<const int*>(sc + (size_t)(((ks0 + (SHIFT ? 0 : u)) >> 2) * TILES + mt) * 256)[fl];
+            xs[i & 1] = SHIFT ? (int)((unsigned)x >> ((ks0 & 3) * 8)) : x;
+        };
+        int ys[NB][SW];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const v4i* f = reinterpret_cast<const v4i*>(frag + (size_t)((ks0 + u) * MT + mt) * 2048) + fl;
-                const v4i lo = f[0], hi = f[64];
-                const v8i x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                int xs = reinterpret_cast<const int*>(sc + (size_t)(((ks0 + (SHIFT ? 0 : u)) >> 2) * MT + mt) * 256)[fl];
-                if constexpr (SHIFT) xs = (int)((unsigned)xs >> ((ks0 & 3) * 8));
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const v8i y = __builtin_shufflevector(b.w[nb][u], b.w[nb][u], 0, 1, 2, 3, -1, -1, -1, -1);
-                    int ys = b.s[nb][u / 4];
-                    if constexpr (SHIFT) ys = (int)((unsigned)ys >> ((ks0 & 3) * 8));
-                    acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, acc[mt][nb], 0, 4, u & 3, xs, u & 3, ys);
-                }
+            for (int d = 0; d < SW; ++d) ys[nb][d] = SHIFT ? (int)((unsigned)b.s[nb][d] >> ((ks0 & 3) * 8)) : b.s[nb][d];
+        fetch(std::integral_constant<int, 0>{});
+        static_for<U * TILES>([&](auto ic) {
+            constexpr int i = decltype(ic)::value, u = i / TILES, mt = i % TILES;
+            if constexpr (i + 1 < U * TILES) fetch(std::integral_constant<int, i + 1>{});
+            if constexpr (TILES > 1) __builtin_amdgcn_sched_barrier(0);
+            const v8i x = __builtin_shufflevector(lo[i & 1], hi[i & 1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const v8i y = __builtin_shufflevector(b.w[nb][u], b.w[nb][u], 0, 1, 2, 3, -1, -1, -1, -1);
+                const v4f c = FIRST && u == 0 ? (v4f){0.f, 0.f, 0.f, 0.f} : acc[mt][nb];
+                acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 4, u & 3, xs[i & 1], u & 3, ys[nb][u / 4]);
             }
         });
     };
+    float iv[MT];
+    float* const op = out + col * ld + n16;
     auto store = [&](int tile) {
+        // column c of lanes holds query c of the tile; the order of the additions is the same for every query, so a score does
+        // not depend on what it is computed together with
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            // column c of lanes is left with query c of the tile, whose fifth digit lies there already: the order of the
-            // additions is the same for every query, so a score does not depend on what it is computed together with
+        for (int nb = 0; nb < NB; ++nb) {
+            const int r = (tile * NB + nb) * 16;
+            float y[MT];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
+            for (int mt = 0; mt < MT; ++mt) {
                 const v4f v = acc[mt][nb];
-                const int r = (tile * NB + nb) * 16 + n16, s = mt * QPT + col;
-                float y = columns_sum(v[0], v[1], v[2], ND == 5 ? 0.f : v[3]);
-                if (ND == 5) y += v[3];
-                if (col < QPT && s < nqh && r < rows) out[(long long)s * ld + r] = y * inv[s];
+                y[mt] = (v[0] + v[1]) + (v[2] + v[3]);
+                if constexpr (L::INSIDE) y[mt] += fifth_digits(v[0], v[1], v[2]);
+                else if constexpr (ND == 5) y[mt] += acc[MT + mt / 4][nb][mt & 3];
+                y[mt] *= iv[mt];
+                asm volatile("" : "+v"(y[mt]));                 // here: else the products sink into the branches below
+            }
+            if (r + n16 < rows && col < QPT) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+                    if (mt * QPT + col < nqh) op[mt * QPT * ld + r] = y[mt];
             }
         }
     };
@@ -499,7 +524,12 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     load(x, t < tiles ? t : tiles - 1, 0);                      // on its way while the queries are split
     mx4_stage_queries<ND, MT, NW * 64>(a, q0, nqh, frag, sc, inv);
     if (first >= tiles) return;
-    clear();
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) iv[mt] = inv[col < QPT ? mt * QPT + col : 0];
+    auto piece = [&](const Buf& b, int ks0) {
+        if (ONE || ks0 == 0) multiply(b, ks0, std::true_type{});
+        else multiply(b, ks0, std::false_type{});
+    };
     for (;;) {
         // where the piece behind this one lies, and the one behind that
         auto next = [&](int& t2, int& k2) {
@@ -514,22 +544,16 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         next(t2, k2);
         load(y, t2 < tiles ? t2 : tiles - 1, k2);
         __builtin_amdgcn_sched_barrier(0);                      // the fetch goes out before the products wait for theirs
-        multiply(x, k);
-        if (k2 == 0) {
-            store(t);
-            clear();
-        }
+        piece(x, k);
+        if (k2 == 0) store(t);
         if (t2 >= tiles) break;
         t = t2;
         k = k2;
         next(t, k);
         load(x, t < tiles ? t : tiles - 1, k);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(y, k2);
-        if (k == 0) {
-            store(t2);
-            clear();
-        }
+        piece(y, k2);
+        if (k == 0) store(t2);
         if (t >= tiles) break;
     }
 }
@@ -540,30 +564,29 @@ struct Mx4Shape {
     bool one, nt;
     size_t lds;
 };
-static size_t mx4_lds(int ks, int u, int mt) {
+static int mx4_tiles(int nd, int mt) { return nd == 5 && mt > 1 ? mt + (mt + 3) / 4 : mt; }        // Mx4Digits::TILES
+static size_t mx4_lds(int ks, int u, int tiles) {
     const int ksu = (ks + u - 1) / u * u;
-    return (size_t)ksu * mt * 2048 + (size_t)(ksu + 3) / 4 * mt * 256 + (size_t)mt * 4 * sizeof(float);
+    return (size_t)ksu * tiles * 2048 + (size_t)(ksu + 3) / 4 * tiles * 256 + (size_t)tiles * 4 * sizeof(float);
 }
 static Mx4Shape mx4_shape(int type, int dim, long long nq) {
     Mx4Shape p = {};
     const int ks = mx4_blocks(dim);
     p.nd = type == RAG_MX4_F32 ? 5 : 4;
-    const int qpt = p.nd == 5 ? 3 : 4;
-    const long long need = (nq + qpt - 1) / qpt;
     auto fetch = [&](int mt) {
         if (mt <= 2) return ks <= 8 ? ks : (ks & 7) == 0 || (ks & 7) > 4 ? 8 : 4;
-        if (mt == 4) return ks <= 4 ? ks : (ks & 3) == 0 ? 4 : (ks & 1) == 0 ? 2 : 1;
+        if (mt == 4) return ks == 3 ? 3 : (ks & 3) == 0 ? 4 : (ks & 1) == 0 ? 2 : 1;
         return (ks & 1) == 0 ? 2 : 1;
     };
-    p.mt = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8;
-    while (p.mt > 1 && mx4_lds(ks, fetch(p.mt), p.mt) > 160 * 1024) p.mt /= 2;
+    p.mt = nq <= (p.nd == 5 ? 3 : 4) ? 1 : nq <= 8 ? 2 : nq <= 16 ? 4 : 8;
+    while (p.mt > 1 && mx4_lds(ks, fetch(p.mt), mx4_tiles(p.nd, p.mt)) > 160 * 1024) p.mt /= 2;
     p.u = fetch(p.mt);
-    p.one = p.u == ks;
+    p.one = p.mt <= 2 && p.u == ks;
     p.nb = p.mt <= 2 ? 1 : 2;
     p.nw = p.mt == 8 ? 8 : 4;
     p.ksu = (ks + p.u - 1) / p.u * p.u;
-    p.qb = p.mt * qpt;
-    p.lds = mx4_lds(ks, p.u, p.mt);
+    p.qb = p.nd == 5 && p.mt == 1 ? 3 : 4 * p.mt;
+    p.lds = mx4_lds(ks, p.u, mx4_tiles(p.nd, p.mt));
     return p;
 }
 
@@ -588,9 +611,8 @@ static int mx4_launch_nd(const Mx4Shape& p, const Mx4ScoreArgs& a, long long gri
     MX4_CASE(MT, 1, 4, 4, false); MX4_CASE(MT, 1, 8, 4, false)
     MX4_FEW(1);
     MX4_FEW(2);
-    MX4_CASE(4, 2, 1, 4, true); MX4_CASE(4, 2, 2, 4, true); MX4_CASE(4, 2, 3, 4, true); MX4_CASE(4, 2, 4, 4, true);
-    MX4_CASE(4, 2, 1, 4, false); MX4_CASE(4, 2, 2, 4, false); MX4_CASE(4, 2, 4, 4, false);
-    MX4_CASE(8, 2, 1, 8, true); MX4_CASE(8, 2, 2, 8, true); MX4_CASE(8, 2, 1, 8, false); MX4_CASE(8, 2, 2, 8, false);
+    MX4_CASE(4, 2, 1, 4, false); MX4_CASE(4, 2, 2, 4, false); MX4_CASE(4, 2, 3, 4, false); MX4_CASE(4, 2, 4, 4, false);
+    MX4_CASE(8, 2, 1, 8, false); MX4_CASE(8, 2, 2, 8, false);
 #undef MX4_FEW
 #undef MX4_CASE
     return fail(RAG_ERR_INVALID, "internal: no four-bit product kernel for this shape");
@@ -630,6 +652,8 @@ static Mx4ScoreArgs mx4_score_args(const rag_mx4_store_t* st, const Mx4Shape& p,
     a.ksu = p.ksu;
     a.code_ld = mx4_code_bytes(st->dim);
     a.scale_ld = mx4_scale_bytes(st->dim);
+    a.code_bytes = (size_t)((st->n + 15) / 16 * 16) * a.code_ld;
+    a.scale_bytes = (size_t)st->n * a.scale_ld;
     a.normalize = normalize;
     a.out = out;
     return a;
@@ -649,10 +673,17 @@ static int mx4_scores(const rag_mx4_store_t* st, long long row0, long long rows,
     const long long unit = 16LL * p.nb * p.nw;                  // rows of one step of a workgroup
     const long long units = (rows + unit - 1) / unit;
     if (a.nqb == 1) return mx4_launch_any(p, a, std::min<long long>(units, getenv("MXG") ? atoi(getenv("MXG")) : p.mt == 8 ? 256 : p.mt == 4 ? 512 : 1024), st->device, s);
-    const long long want = std::max<long long>(1, 2048 / a.nqb);                          // slabs
-    a.slab = (units + want - 1) / want * unit;
-    const long long slabs = (rows + a.slab - 1) / a.slab;
-    return mx4_launch_any(p, a, (slabs + 7) / 8 * 8 * a.nqb, st->device, s);
+    // Slabs: as many as make the workgroups come out even over the chip's compute units, each long against the staging of
+    // its queries (about two units of work)
+    const long long seats = 256LL * (p.mt == 8 ? 1 : 2);
+    long long best = 1, least = LLONG_MAX;
+    for (long long n = 1; n <= std::min<long long>(units, std::max<long long>(64, 8 * seats / a.nqb)); ++n) {
+        const long long cost = (n * a.nqb + seats - 1) / seats * ((units + n - 1) / n + 2);
+        if (cost < least) { least = cost; best = n; }
+    }
+    a.slab = (units + best - 1) / best * unit;
+    a.slabs = (rows + a.slab - 1) / a.slab;
+    return mx4_launch_any(p, a, (a.slabs * a.nqb + 7) / 8 * 8, st->device, s);
 }
 
 int direct_select_segments(long long nq, long long n_row, long long seg_rows, int k, float min_score, const uint8_t* mask,
