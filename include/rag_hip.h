@@ -466,7 +466,7 @@ int rag_mx4_layout(int dim, int64_t* code_bytes, int64_t* scale_bytes);
 /* Quantise `count` rows of x_dev (elements of x_type, x_stride elements from row to row) as they are written:
  *   rows_dev NULL   to the rows [first, first + count)
  *   rows_dev        to the positions it names; a position outside [0, n) is skipped, of several rows for one position the last is
- *                   kept.  owner_dev: n int32, zero before the first such call; the call leaves them zero.
+ *                   kept.  owner_dev: n int32, zero before the first such call; every call leaves them zero.
  *   normalize       1: every row is divided by its norm first (COSINE; sum of squares in fp64; a zero row stays zero) */
 int rag_mx4_write_device(const rag_mx4_store_t* st, int64_t first, const int64_t* rows_dev, int32_t* owner_dev, int64_t count,
                          const void* x_dev, int x_type, int64_t x_stride, int normalize, void* stream);

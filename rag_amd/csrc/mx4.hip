@@ -35,13 +35,16 @@ typedef unsigned v2u __attribute__((ext_vector_type(2)));
 
 struct Mx4DeviceGuard {
     int prev = -1;
-    bool ok = true;
+    bool ok = true, moved = false;
     explicit Mx4DeviceGuard(int dev) {
         if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-        if (prev != dev) ok = (hipSetDevice(dev) == hipSuccess);
+        if (prev != dev) {
+            moved = true;
+            ok = hipSetDevice(dev) == hipSuccess;
+        }
     }
     ~Mx4DeviceGuard() {
-        if (prev >= 0) (void)hipSetDevice(prev);
+        if (moved && prev >= 0) (void)hipSetDevice(prev);
     }
 };
 
@@ -66,20 +69,23 @@ __device__ __forceinline__ float mx4_elem(const void* row, int type, long long i
     const unsigned short h = static_cast<const unsigned short*>(row)[i];
     return type == RAG_MX4_BF16 ? bf16_f32(h) : f16_f32(h);
 }
-// N (4 or 8) consecutive elements from i on; past `dim` zero.  vec: rows start on 16-byte boundaries.
-template <int N>
+// N (4 or 8) consecutive elements from i on; past `dim` zero.  vec: rows start on 16-byte boundaries.  ONCE: read past the
+// caches' retention, for rows that nobody reads again (writing 100k rows of 384 fp32: 43 -> 35 us).
+template <int N, bool ONCE = false>
 __device__ __forceinline__ void mx4_load(const void* row, int type, int i, int dim, int vec, float* v) {
     if (vec && i + N <= dim) {
         if (type == RAG_MX4_F32) {
 #pragma unroll
             for (int j = 0; j < N; j += 4) {
-                const v4f x = *reinterpret_cast<const v4f*>(static_cast<const float*>(row) + i + j);
+                const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(row) + i + j);
+                const v4f x = ONCE ? __builtin_nontemporal_load(p) : *p;
                 v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
             }
         } else {
             unsigned w[N / 2];
             if constexpr (N == 8) {
-                const v4i x = *reinterpret_cast<const v4i*>(static_cast<const unsigned short*>(row) + i);
+                const v4i* p = reinterpret_cast<const v4i*>(static_cast<const unsigned short*>(row) + i);
+                const v4i x = ONCE ? __builtin_nontemporal_load(p) : *p;
                 w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
             } else {
                 const v2u x = *reinterpret_cast<const v2u*>(static_cast<const unsigned short*>(row) + i);
@@ -125,21 +131,26 @@ __device__ __forceinline__ float wave_inv_norm(const void* row, int type, int di
 
 // ------------------------------------------------------------------------------------------------ writing rows
 // Bound by HBM: dim * size bytes in, 0.53 dim bytes out per row.  A lane takes 8 consecutive elements, four lanes a group:
-// loads of 16 (two for fp32) and stores of 4 bytes per lane, both contiguous over the wave.
+// loads of 16 (two for fp32) and stores of 4 bytes per lane, both contiguous over the wave; the loads of four such units
+// are under way at once.
 struct Mx4WriteArgs {
     uint8_t* codes;
     uint8_t* scales;
     long long n;                 // rows of the store
     const long long* rows;       // nullptr: row `first + i`
-    int* owner;                  // with rows: owner[r] = 1 + the last i that names row r (mx4_claim_kernel)
+    int* owner;                  // nullptr, or owner[r] = 1 + the last i that names row r (mx4_claim_kernel)
     long long first;
     long long count;
     const void* x;
     long long ldx;               // elements
-    int type, dim, ks, code_ld, scale_ld, normalize, vec;
+    int dim, code_ld, scale_ld, normalize;
+    int upr;                     // units of 8 elements per (padded) row
+    unsigned per;                // ceil(2^32 / upr): u / upr == (u * per) >> 32 for the units of a workgroup
     int per_block;               // rows a workgroup takes
 };
-constexpr int MX4_WRITE_ROWS = 64;           // most rows of one workgroup
+constexpr int MX4_ROWS = 64;                 // most rows of one workgroup
+constexpr int MX4_FEW = 256;                 // up to so many positions a workgroup looks for repeated ones itself
+constexpr int MX4_UNITS = 4;
 
 // A position that is named twice keeps the last of its rows: the highest index wins the claim, whatever the order of arrival.
 __global__ __launch_bounds__(256) void mx4_claim_kernel(const long long* rows, long long count, long long n, int* owner) {
@@ -149,63 +160,91 @@ __global__ __launch_bounds__(256) void mx4_claim_kernel(const long long* rows, l
     if (r >= 0 && r < n) atomicMax(&owner[r], (int)(i + 1));
 }
 
+// AT: rows go to named positions, and those that are skipped are not fetched (for consecutive rows the test would cost 10 %)
+template <int TYPE, bool VEC, bool AT>
 __global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
-    __shared__ long long s_to[MX4_WRITE_ROWS];
-    __shared__ float s_inv[MX4_WRITE_ROWS];
+    __shared__ long long s_to[MX4_ROWS];
+    __shared__ float s_inv[MX4_ROWS];
+    __shared__ int s_late[MX4_ROWS];
     const long long i0 = (long long)blockIdx.x * a.per_block;
     const int nr = (int)(a.count - i0 < a.per_block ? a.count - i0 : a.per_block);
     const int tid = threadIdx.x, lane = tid & 63;
-    const size_t esize = a.type == RAG_MX4_F32 ? 4 : 2;
+    constexpr size_t ESIZE = TYPE == RAG_MX4_F32 ? 4 : 2;
+    const char* x = static_cast<const char*>(a.x) + (size_t)i0 * a.ldx * ESIZE;
     if (tid < nr) {
         long long to = a.first + i0 + tid;
-        if (a.rows) {
+        if (AT) {
             to = a.rows[i0 + tid];
             if (to < 0 || to >= a.n) to = -1;
-            else if (a.owner[to] != (int)(i0 + tid + 1)) to = -1;
-            else a.owner[to] = 0;           // only the winner sees its own number here, so no other row is misled by the reset
+            else if (a.owner) {
+                if (a.owner[to] != (int)(i0 + tid + 1)) to = -1;
+                else a.owner[to] = 0;       // only the winner sees its own number here, so no other row is misled by the reset
+            }
         }
         s_to[tid] = to;
         s_inv[tid] = 1.f;
+        s_late[tid] = 0;
     }
     __syncthreads();
+    if (AT && !a.owner && a.count > 1) {                     // at most MX4_FEW positions: does a later row name the same one?
+        const long long mine = tid < a.count ? a.rows[tid] : -1;
+        for (int r = 0; r < nr; ++r)
+            if (mine >= 0 && mine == s_to[r] && tid > i0 + r) s_late[r] = 1;
+        __syncthreads();
+        if (tid < nr && s_late[tid]) s_to[tid] = -1;
+        __syncthreads();
+    }
     if (a.normalize) {
         for (int r = tid >> 6; r < nr; r += 4) {
-            const float inv = wave_inv_norm(static_cast<const char*>(a.x) + (size_t)(i0 + r) * a.ldx * esize, a.type, a.dim, lane);
+            const float inv = wave_inv_norm(x + (size_t)r * a.ldx * ESIZE, TYPE, a.dim, lane);
             if (lane == 0) s_inv[r] = inv;
         }
         __syncthreads();
     }
-    const int upr = a.ks * 16;                                   // units of 8 elements per (padded) row
-    for (int u = tid; u < nr * upr; u += 256) {
-        const int r = u / upr, c = u - r * upr;
-        const long long to = s_to[r];
-        if (to < 0) continue;                                    // uniform over the four lanes of a group
-        float v[8];
-        mx4_load<8>(static_cast<const char*>(a.x) + (size_t)(i0 + r) * a.ldx * esize, a.type, c * 8, a.dim, a.vec, v);
-        unsigned most = 0;
+    const int units = nr * a.upr;
+    for (int u0 = tid; u0 < units; u0 += 256 * MX4_UNITS) {
+        float v[MX4_UNITS][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (a.normalize) v[j] *= s_inv[r];
-            const unsigned m = __float_as_uint(v[j]) & 0x7fffffffu;
-            most = m > most ? m : most;
+        for (int j = 0; j < MX4_UNITS; ++j) {
+            const int u = u0 + 256 * j < units ? u0 + 256 * j : u0;
+            const int r = (int)__umulhi((unsigned)u, a.per), c = u - r * a.upr;
+            if (!AT || s_to[r] >= 0) mx4_load<8, true>(x + (size_t)r * a.ldx * ESIZE, TYPE, c * 8, a.dim, VEC, v[j]);
         }
-        most = quad_max(most);
-        // scale: floor(log2(most)) - 2, one more where most / 2^floor > 1.75 (then 6 is nearer than the 8 that four bits lack)
-        int e = (int)(most >> 23) - 129 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);
-        e = e < -126 ? -126 : e > 125 ? 125 : e;
-        const bool bad = most >= 0x7f800000u;                    // a NaN or an infinity: the group is NaN
-        const float scale = mx4_pow2(e);
-        unsigned w = 0;
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], scale, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
-        *reinterpret_cast<unsigned*>(a.codes + mx4_code_at(to, a.code_ld, c >> 4) + (c & 15) * 4) = bad ? 0u : w;
-        if ((c & 3) == 0) a.scales[(size_t)to * a.scale_ld + mx4_scale_at(c >> 2)] = bad ? 255 : (uint8_t)(e + 127);
+#pragma unroll
+        for (int j = 0; j < MX4_UNITS; ++j) {
+            const int u = u0 + 256 * j;
+            if (u >= units) break;
+            const int r = (int)__umulhi((unsigned)u, a.per), c = u - r * a.upr;
+            const long long to = s_to[r];
+            if (AT && to < 0) continue;                                // uniform over the four lanes of a group
+            const float inv = s_inv[r];
+            unsigned most = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[j][i] *= inv;
+                const unsigned m = __float_as_uint(v[j][i]) & 0x7fffffffu;
+                most = m > most ? m : most;
+            }
+            most = quad_max(most);
+            // scale: floor(log2(most)) - 2, one more where most / 2^floor > 1.75 (then 6 is nearer than the 8 that four bits lack)
+            int e = (int)(most >> 23) - 129 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);
+            e = e < -126 ? -126 : e > 125 ? 125 : e;
+            const bool bad = most >= 0x7f800000u;                // a NaN or an infinity: the group is NaN
+            const float scale = mx4_pow2(e);
+            unsigned w = 0;
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[j][0], v[j][1], scale, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[j][2], v[j][3], scale, 1);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[j][4], v[j][5], scale, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[j][6], v[j][7], scale, 3);
+            *reinterpret_cast<unsigned*>(a.codes + mx4_code_at(to, a.code_ld, c >> 4) + (c & 15) * 4) = bad ? 0u : w;
+            if ((c & 3) == 0) a.scales[(size_t)to * a.scale_ld + mx4_scale_at(c >> 2)] = bad ? 255 : (uint8_t)(e + 127);
+        }
     }
 }
 
 // ------------------------------------------------------------------------------------------------ reading rows
+// Bound by HBM, mostly by what it writes.  A lane makes 8 elements from 4 bytes of codes and a scale; four such units are under
+// way at once, behind one fetch of the workgroup's positions.
 struct Mx4ReadArgs {
     const uint8_t* codes;
     const uint8_t* scales;
@@ -213,7 +252,9 @@ struct Mx4ReadArgs {
     const long long* rows;
     long long count;
     void* out;                   // [count][dim]
-    int type, dim, ks, code_ld, scale_ld, vec;
+    int dim, code_ld, scale_ld;
+    int upr;
+    unsigned per;                // as for writing; not used where upr is 1
     int per_block;
 };
 
@@ -231,39 +272,63 @@ __device__ __forceinline__ unsigned pack16(int type, float lo, float hi) {
     return (unsigned)a | ((unsigned)b << 16);
 }
 
+template <int TYPE, bool VEC>
 __global__ __launch_bounds__(256) void mx4_read_kernel(Mx4ReadArgs a) {
+    __shared__ long long s_from[MX4_ROWS];
     const long long i0 = (long long)blockIdx.x * a.per_block;
     const int nr = (int)(a.count - i0 < a.per_block ? a.count - i0 : a.per_block);
-    const int upr = (a.dim + 7) / 8;
-    for (int u = threadIdx.x; u < nr * upr; u += 256) {
-        const int r = u / upr, c = u - r * upr;
-        const long long from = a.rows[i0 + r];
-        float v[8] = {};
-        if (from >= 0 && from < a.n) {
-            const unsigned w = *reinterpret_cast<const unsigned*>(a.codes + mx4_code_at(from, a.code_ld, c >> 4) + (c & 15) * 4);
-            const unsigned b = a.scales[(size_t)from * a.scale_ld + mx4_scale_at(c >> 2)];
-            const float f = b == 255 ? NAN : b == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(b << 23);
-            v2f p;
-            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0); v[0] = p.x * f; v[1] = p.y * f;
-            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1); v[2] = p.x * f; v[3] = p.y * f;
-            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2); v[4] = p.x * f; v[5] = p.y * f;
-            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3); v[6] = p.x * f; v[7] = p.y * f;
-        }
-        const size_t at = (size_t)(i0 + r) * a.dim + (size_t)c * 8;
-        if (a.vec) {
-            if (a.type == RAG_MX4_F32) {
-                v4f* o = reinterpret_cast<v4f*>(static_cast<float*>(a.out) + at);
-                o[0] = (v4f){v[0], v[1], v[2], v[3]};
-                o[1] = (v4f){v[4], v[5], v[6], v[7]};
-            } else {
-                *reinterpret_cast<v4i*>(static_cast<unsigned short*>(a.out) + at) =
-                    (v4i){(int)pack16(a.type, v[0], v[1]), (int)pack16(a.type, v[2], v[3]), (int)pack16(a.type, v[4], v[5]),
-                          (int)pack16(a.type, v[6], v[7])};
+    const int tid = threadIdx.x;
+    if (tid < nr) {
+        const long long from = a.rows[i0 + tid];
+        s_from[tid] = from >= 0 && from < a.n ? from : -1;
+    }
+    __syncthreads();
+    const int units = nr * a.upr;
+    for (int u0 = tid; u0 < units; u0 += 256 * MX4_UNITS) {
+        unsigned w[MX4_UNITS];
+        int b[MX4_UNITS];
+#pragma unroll
+        for (int j = 0; j < MX4_UNITS; ++j) {
+            const int u = u0 + 256 * j < units ? u0 + 256 * j : u0;
+            const int r = a.upr == 1 ? u : (int)__umulhi((unsigned)u, a.per), c = u - r * a.upr;
+            const long long from = s_from[r];
+            w[j] = 0;
+            b[j] = 127;
+            if (from >= 0) {
+                w[j] = *reinterpret_cast<const unsigned*>(a.codes + mx4_code_at(from, a.code_ld, c >> 4) + (c & 15) * 4);
+                b[j] = a.scales[(size_t)from * a.scale_ld + mx4_scale_at(c >> 2)];
             }
-        } else {
-            for (int j = 0; j < 8 && c * 8 + j < a.dim; ++j) {
-                if (a.type == RAG_MX4_F32) static_cast<float*>(a.out)[at + j] = v[j];
-                else static_cast<unsigned short*>(a.out)[at + j] = (unsigned short)pack16(a.type, v[j], 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < MX4_UNITS; ++j) {
+            const int u = u0 + 256 * j;
+            if (u >= units) break;
+            const int r = a.upr == 1 ? u : (int)__umulhi((unsigned)u, a.per), c = u - r * a.upr;
+            const float f = b[j] == 255 ? NAN : b[j] == 0 ? __uint_as_float(0x00400000u) : __uint_as_float((unsigned)b[j] << 23);
+            float v[8];
+            v2f p;
+            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], 1.f, 0); v[0] = p.x * f; v[1] = p.y * f;
+            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], 1.f, 1); v[2] = p.x * f; v[3] = p.y * f;
+            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], 1.f, 2); v[4] = p.x * f; v[5] = p.y * f;
+            p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], 1.f, 3); v[6] = p.x * f; v[7] = p.y * f;
+            const size_t at = (size_t)(i0 + r) * a.dim + (size_t)c * 8;
+            if constexpr (VEC) {
+                if constexpr (TYPE == RAG_MX4_F32) {
+                    v4f* o = reinterpret_cast<v4f*>(static_cast<float*>(a.out) + at);
+                    o[0] = (v4f){v[0], v[1], v[2], v[3]};
+                    o[1] = (v4f){v[4], v[5], v[6], v[7]};
+                } else {
+                    *reinterpret_cast<v4i*>(static_cast<unsigned short*>(a.out) + at) =
+                        (v4i){(int)pack16(TYPE, v[0], v[1]), (int)pack16(TYPE, v[2], v[3]), (int)pack16(TYPE, v[4], v[5]),
+                              (int)pack16(TYPE, v[6], v[7])};
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (c * 8 + i < a.dim) {
+                        if constexpr (TYPE == RAG_MX4_F32) static_cast<float*>(a.out)[at + i] = v[i];
+                        else static_cast<unsigned short*>(a.out)[at + i] = (unsigned short)pack16(TYPE, v[i], 0.f);
+                    }
             }
         }
     }
@@ -302,9 +367,10 @@ struct Mx4Digits {
     static constexpr int QPT = INSIDE ? 3 : 4;                   // queries per tile of 16 eight-bit rows
 };
 
-// queries [q0, q0 + nqh) -> digit fragments in LDS.  frag[(block * TILES + tile) * 2 + half][lane][16 bytes], then the scales
+// queries [q0, q0 + nqh) -> digit fragments in LDS.  frag[(block * TILES + tile) * 2 + half][place of lane][16 bytes], then the scales
 // sc[(block / 4) * TILES + tile][lane][block % 4], then 1 / |q|.  Blocks past the row's are zero: they meet a real block of the
-// row again.  What the fragments of absent queries hold does not matter: it stays in result rows that nobody reads.
+// row again.  A lane's place: its row number exclusive-or'ed with column and half, so that the lanes that write one digit of
+// consecutive elements meet different banks (with the rows in order sixteen lanes shared four).  What the fragments of absent queries hold does not matter: it stays in result rows that nobody reads.
 template <int ND, int MT, int NT>
 __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long long q0, int nqh, uint8_t* frag, uint8_t* sc, float* inv) {
     typedef Mx4Digits<ND, MT> L;
@@ -326,8 +392,9 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long lo
         if ((tid & 63) == 0) inv[s] = f;
     }
     const int upq = a.ks * 32;                                  // units of 4 elements per query
-    for (int u = tid; u < nqh * upq; u += NT) {
-        const int s = u / upq, c = u - s * upq;
+    for (int s = 0, c = tid;; c += NT) {
+        while (c >= upq && s < nqh) { c -= upq; ++s; }
+        if (s >= nqh) break;
         float v[4];
         mx4_load<4>(q + (size_t)s * a.ldq * esize, a.q_type, c * 4, a.dim, a.q_vec, v);
         unsigned most = 0;
@@ -346,6 +413,7 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long lo
         const int col = (in >> 2) & 3, half = in >> 4;
         const int tile = s / QPT, slot = s - tile * QPT;
         uint8_t* to = frag + (size_t)(block * TILES * 2 + half) * 1024 + col * 256 + (in & 3) * 4;
+        const int turn = col | half << 2;
         uint8_t* ts = sc + (size_t)((block >> 2) * TILES) * 256 + (in >> 3) * 64 + (block & 3);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] *= down;
@@ -362,7 +430,7 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long lo
             if (bad) p = d == 0 ? 0x7f7f7f7f : 0;               // NaN: every score of the query is NaN
             const int m = d < 4 ? 4 * slot + d : L::INSIDE ? 12 + slot : 4 * slot + (tile & 3);
             const int at = d < 4 || L::INSIDE ? tile : MT + (tile >> 2);
-            *reinterpret_cast<int*>(to + at * 2048 + m * 16) = p;
+            *reinterpret_cast<int*>(to + at * 2048 + (m ^ turn) * 16) = p;
             if ((in & 7) == 0) ts[at * 256 + m * 4] = (uint8_t)(127 + e - 5 * d);
         }
     }
@@ -461,35 +529,37 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         constexpr bool FIRST = decltype(first_of_row)::value;   // begins the sums at zero
         constexpr bool SHIFT = !ONE && U < 4;                   // the fetch may begin inside a scale dword
         const uint8_t* f = frag + (size_t)ks0 * TILES * 2048;
-        int fl = lane;
-        if constexpr (TILES > 1) asm volatile("" : "+v"(fl));      // more than one tile's fragments do not fit the registers: read from LDS each time
-        // query fragments one tile ahead: the LDS latency passes under the products of the tile before
-        v4i lo[2], hi[2];
-        int xs[2];
+        int fl = (col * 16 + (n16 ^ col)) * 16, sl = lane * 4;     // places of the first half; the second half's differ in bit 2 of the row
+        if constexpr (TILES > 1) asm volatile("" : "+v"(fl), "+v"(sl));      // more than one tile's fragments do not fit the registers: read from LDS each time
+        // query fragments AHEAD tiles ahead: the LDS latency passes under the products of the tiles before
+        constexpr int AHEAD = 2, RING = AHEAD + 1;
+        v4i lo[RING], hi[RING];
+        int xs[RING];
         auto fetch = [&](auto ic) {
             constexpr int i = decltype(ic)::value, u = i / TILES, mt = i % TILES;
-            const v4i* p = reinterpret_cast<const v4i*>(f + i * 2048) + fl;
-            lo[i & 1] = p[0];
-            hi[i & 1] = p[64];
-            const int x = reinterpret_cast<const int*>(sc + (size_t)(((ks0 + (SHIFT ? 0 : u)) >> 2) * TILES + mt) * 256)[fl];
-            xs[i & 1] = SHIFT ? (int)((unsigned)x >> ((ks0 & 3) * 8)) : x;
+            lo[i % RING] = *reinterpret_cast<const v4i*>(f + i * 2048 + fl);
+            hi[i % RING] = *reinterpret_cast<const v4i*>(f + i * 2048 + 1024 + (fl ^ 64));
+            const int x = *reinterpret_cast<const int*>(sc + (size_t)(((ks0 + (SHIFT ? 0 : u)) >> 2) * TILES + mt) * 256 + sl);
+            xs[i % RING] = SHIFT ? (int)((unsigned)x >> ((ks0 & 3) * 8)) : x;
         };
         int ys[NB][SW];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int d = 0; d < SW; ++d) ys[nb][d] = SHIFT ? (int)((unsigned)b.s[nb][d] >> ((ks0 & 3) * 8)) : b.s[nb][d];
-        fetch(std::integral_constant<int, 0>{});
+        static_for<AHEAD>([&](auto ic) {
+            if constexpr (decltype(ic)::value < U * TILES) fetch(ic);
+        });
         static_for<U * TILES>([&](auto ic) {
             constexpr int i = decltype(ic)::value, u = i / TILES, mt = i % TILES;
-            if constexpr (i + 1 < U * TILES) fetch(std::integral_constant<int, i + 1>{});
+            if constexpr (i + AHEAD < U * TILES) fetch(std::integral_constant<int, i + AHEAD>{});
             if constexpr (TILES > 1) __builtin_amdgcn_sched_barrier(0);
-            const v8i x = __builtin_shufflevector(lo[i & 1], hi[i & 1], 0, 1, 2, 3, 4, 5, 6, 7);
+            const v8i x = __builtin_shufflevector(lo[i % RING], hi[i % RING], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const v8i y = __builtin_shufflevector(b.w[nb][u], b.w[nb][u], 0, 1, 2, 3, -1, -1, -1, -1);
                 const v4f c = FIRST && u == 0 ? (v4f){0.f, 0.f, 0.f, 0.f} : acc[mt][nb];
-                acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 4, u & 3, xs[i & 1], u & 3, ys[nb][u / 4]);
+                acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 4, u & 3, xs[i % RING], u & 3, ys[nb][u / 4]);
             }
         });
     };
@@ -582,8 +652,8 @@ static Mx4Shape mx4_shape(int type, int dim, long long nq) {
     while (p.mt > 1 && mx4_lds(ks, fetch(p.mt), mx4_tiles(p.nd, p.mt)) > 160 * 1024) p.mt /= 2;
     p.u = fetch(p.mt);
     p.one = p.mt <= 2 && p.u == ks;
-    p.nb = p.mt <= 2 ? 1 : 2;
-    p.nw = p.mt == 8 ? 8 : 4;
+    p.nb = p.mt <= 4 ? 1 : 2;
+    p.nw = p.mt >= 4 ? 8 : 4;
     p.ksu = (ks + p.u - 1) / p.u * p.u;
     p.qb = p.nd == 5 && p.mt == 1 ? 3 : 4 * p.mt;
     p.lds = mx4_lds(ks, p.u, mx4_tiles(p.nd, p.mt));
@@ -611,7 +681,7 @@ static int mx4_launch_nd(const Mx4Shape& p, const Mx4ScoreArgs& a, long long gri
     MX4_CASE(MT, 1, 4, 4, false); MX4_CASE(MT, 1, 8, 4, false)
     MX4_FEW(1);
     MX4_FEW(2);
-    MX4_CASE(4, 2, 1, 4, false); MX4_CASE(4, 2, 2, 4, false); MX4_CASE(4, 2, 3, 4, false); MX4_CASE(4, 2, 4, 4, false);
+    MX4_CASE(4, 1, 1, 8, false); MX4_CASE(4, 1, 2, 8, false); MX4_CASE(4, 1, 3, 8, false); MX4_CASE(4, 1, 4, 8, false);
     MX4_CASE(8, 2, 1, 8, false); MX4_CASE(8, 2, 2, 8, false);
 #undef MX4_FEW
 #undef MX4_CASE
@@ -638,6 +708,11 @@ static int mx4_check_type(int type) {
 static size_t mx4_esize(int type) { return type == RAG_MX4_F32 ? 4 : 2; }
 static int mx4_aligned(const void* p, long long ld, int type) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (size_t)ld * mx4_esize(type) % 16 == 0;
+}
+// rows of a workgroup that writes or reads rows: four units a thread, fewer where that would leave compute units without work
+static int mx4_rows_per_block(long long count, int upr) {
+    const long long full = std::max(1, std::min(MX4_ROWS, 256 * MX4_UNITS / upr));
+    return (int)std::max<long long>(1, std::min<long long>(full, count / 512));
 }
 static Mx4ScoreArgs mx4_score_args(const rag_mx4_store_t* st, const Mx4Shape& p, const void* q, int q_type, long long ldq, int normalize, float* out) {
     Mx4ScoreArgs a = {};
@@ -765,24 +840,33 @@ int rag_mx4_write_device(const rag_mx4_store_t* st, int64_t first, const int64_t
     a.scales = static_cast<uint8_t*>(st->scales);
     a.n = st->n;
     a.rows = reinterpret_cast<const long long*>(rows_dev);
-    a.owner = owner_dev;
     a.first = first;
     a.count = count;
     a.x = x_dev;
     a.ldx = x_stride;
-    a.type = x_type;
     a.dim = st->dim;
-    a.ks = mx4_blocks(st->dim);
     a.code_ld = mx4_code_bytes(st->dim);
     a.scale_ld = mx4_scale_bytes(st->dim);
     a.normalize = normalize ? 1 : 0;
-    a.vec = mx4_aligned(x_dev, x_stride, x_type);
-    a.per_block = std::max(1, std::min(MX4_WRITE_ROWS, 1024 / (a.ks * 16)));
-    if (rows_dev) {
-        hipLaunchKernelGGL(mx4_claim_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, a.rows, (long long)count, a.n, a.owner);
+    a.upr = mx4_blocks(st->dim) * 16;
+    a.per = (unsigned)((0x100000000ull + a.upr - 1) / a.upr);
+    a.per_block = mx4_rows_per_block(count, a.upr);
+    if (rows_dev && count > MX4_FEW) {
+        hipLaunchKernelGGL(mx4_claim_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, a.rows, (long long)count, a.n, owner_dev);
         RAG_HIP_CHECK(hipGetLastError());
+        a.owner = owner_dev;
     }
-    hipLaunchKernelGGL(mx4_write_kernel, dim3((unsigned)((count + a.per_block - 1) / a.per_block)), dim3(256), 0, s, a);
+    const dim3 grid((unsigned)((count + a.per_block - 1) / a.per_block));
+    const int vec = mx4_aligned(x_dev, x_stride, x_type);
+#define MX4_WRITE(T) \
+    if (x_type == T) { \
+        if (rows_dev && vec) hipLaunchKernelGGL((mx4_write_kernel<T, true, true>), grid, dim3(256), 0, s, a); \
+        else if (rows_dev) hipLaunchKernelGGL((mx4_write_kernel<T, false, true>), grid, dim3(256), 0, s, a); \
+        else if (vec) hipLaunchKernelGGL((mx4_write_kernel<T, true, false>), grid, dim3(256), 0, s, a); \
+        else hipLaunchKernelGGL((mx4_write_kernel<T, false, false>), grid, dim3(256), 0, s, a); \
+    }
+    MX4_WRITE(RAG_MX4_F32) MX4_WRITE(RAG_MX4_BF16) MX4_WRITE(RAG_MX4_F16)
+#undef MX4_WRITE
     RAG_HIP_CHECK(hipGetLastError());
     return RAG_OK;
 }
@@ -803,15 +887,22 @@ int rag_mx4_read_device(const rag_mx4_store_t* st, const int64_t* rows_dev, int6
     a.rows = reinterpret_cast<const long long*>(rows_dev);
     a.count = count;
     a.out = out_dev;
-    a.type = out_type;
     a.dim = st->dim;
-    a.ks = mx4_blocks(st->dim);
     a.code_ld = mx4_code_bytes(st->dim);
     a.scale_ld = mx4_scale_bytes(st->dim);
-    a.vec = st->dim % 8 == 0 && mx4_aligned(out_dev, st->dim, out_type);
-    a.per_block = std::max(1, std::min(MX4_WRITE_ROWS, 1024 / ((st->dim + 7) / 8)));
-    hipLaunchKernelGGL(mx4_read_kernel, dim3((unsigned)((count + a.per_block - 1) / a.per_block)), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), a);
+    a.upr = (st->dim + 7) / 8;
+    a.per = (unsigned)((0x100000000ull + a.upr - 1) / a.upr);
+    a.per_block = mx4_rows_per_block(count, a.upr);
+    const dim3 grid((unsigned)((count + a.per_block - 1) / a.per_block));
+    const int vec = st->dim % 8 == 0 && mx4_aligned(out_dev, st->dim, out_type);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+#define MX4_READ(T) \
+    if (out_type == T) { \
+        if (vec) hipLaunchKernelGGL((mx4_read_kernel<T, true>), grid, dim3(256), 0, s, a); \
+        else hipLaunchKernelGGL((mx4_read_kernel<T, false>), grid, dim3(256), 0, s, a); \
+    }
+    MX4_READ(RAG_MX4_F32) MX4_READ(RAG_MX4_BF16) MX4_READ(RAG_MX4_F16)
+#undef MX4_READ
     RAG_HIP_CHECK(hipGetLastError());
     return RAG_OK;
 }
@@ -865,7 +956,7 @@ int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngro
     for (long long g = 0; g < ngroups; ++g)
         work += (groups[4 * g + 1] - groups[4 * g] + p.qb - 1) / p.qb * (groups[4 * g + 3] - groups[4 * g + 2]);
     const long long unit = 16LL * p.nb * p.nw;
-    const long long part = std::max<long long>(2 * unit, std::min<long long>(8192, (work / 2048 + unit - 1) / unit * unit));
+    const long long part = std::max<long long>(4 * unit, std::min<long long>(8192, (work / 1024 + unit - 1) / unit * unit));
     long long m = 0;
     Mx4Item* items = static_cast<Mx4Item*>(items_out);
     long long at = 0;

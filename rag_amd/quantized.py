@@ -62,7 +62,7 @@ class GroupPlan:
             g = g.reshape(0, 4)
         if g.ndim != 2 or g.shape[1] != 4:
             raise ValueError("groups must be [n, 4]: query begin, query end, row begin, row end")
-        self.nq, self.n, self.type, self.device = int(nq), int(n), _type_of(dtype), int(device)
+        self.nq, self.n, self.dim, self.type, self.device = int(nq), int(n), int(dim), _type_of(dtype), int(device)
         self.shapes = np.stack([g[:, 1] - g[:, 0], g[:, 3] - g[:, 2]], 1)
         self.out_begin = np.zeros(g.shape[0], dtype=np.int64)
         count, total, widest = C.c_int64(0), C.c_int64(0), C.c_int32(0)
@@ -154,27 +154,31 @@ class QuantizedIndex:
 
     # -------------------------------------------------------------------- ingest
     def _rows_in(self, x, what="rows"):
-        """x as a device matrix [n, dim] whose rows may lie apart (inner stride 1)."""
-        if _is_torch_cuda(x):
-            if x.device.index != self.device:
+        """x as a device matrix [n, dim] whose rows may lie apart (inner stride 1): (x, n, elements from row to row, type)."""
+        if isinstance(x, torch.Tensor) and x.is_cuda:
+            if x.get_device() != self.device:
                 raise ValueError("tensor is on another device than the index")
-            _type_of(x.dtype)
         else:
-            x = torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32))
-        if x.dim() == 1:
+            x = torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32)).to(self._dev)
+        kind = _TYPES.get(x.dtype)
+        if kind is None:
+            raise ValueError(f"expected float32, bfloat16 or float16, got {x.dtype}")
+        shape = x.shape
+        if len(shape) == 1:
             x = x[None, :]
-        if x.dim() != 2 or x.shape[1] != self.dim:
-            raise ValueError(f"expected {what} [n, {self.dim}], got {tuple(x.shape)}")
-        if not x.is_cuda:
-            x = x.to(self._dev)
-        if x.shape[0] and (x.stride(1) != 1 and self.dim > 1 or x.stride(0) < self.dim and x.shape[0] > 1):
-            x = x.contiguous()
-        return x, max(x.stride(0), self.dim)
+            shape = x.shape
+        if len(shape) != 2 or shape[1] != self.dim:
+            raise ValueError(f"expected {what} [n, {self.dim}], got {tuple(shape)}")
+        if x.is_contiguous():
+            return x, shape[0], self.dim, kind
+        if x.stride(1) == 1 and x.stride(0) >= self.dim:
+            return x, shape[0], x.stride(0), kind
+        return x.contiguous(), shape[0], self.dim, kind
 
     def add(self, x) -> None:
         """Append rows (numpy, or a CUDA tensor in float32, bfloat16 or float16), quantised as they are written."""
-        x, ld = self._rows_in(x)
-        first, count = self._n, x.shape[0]
+        x, count, ld, kind = self._rows_in(x)
+        first = self._n
         if count == 0:
             return
         have = 0 if self._codes is None else self._codes.shape[0]
@@ -184,34 +188,34 @@ class QuantizedIndex:
         if self._active is not None:
             self._active = torch.cat([self._active, torch.ones((count,), dtype=torch.uint8, device=self._dev)])
         self._renew()
-        self._write(first, None, count, x, ld)
+        self._write(first, None, count, x, ld, kind)
 
     def write(self, rows, x) -> None:
         """Replace rows.  ``rows``: the first of consecutive positions (int), or one position per row of ``x`` (numpy, or
         a CUDA int64 tensor); a position outside the index is skipped, of several rows for one position the last is kept."""
-        x, ld = self._rows_in(x)
+        x, count, ld, kind = self._rows_in(x)
         if isinstance(rows, (int, np.integer)):
-            if not 0 <= int(rows) <= self._n - x.shape[0]:
+            if not 0 <= int(rows) <= self._n - count:
                 raise ValueError("the rows do not lie inside the index")
-            self._write(int(rows), None, x.shape[0], x, ld)
+            self._write(int(rows), None, count, x, ld, kind)
             return
         at = self._positions(rows)
-        if at.numel() != x.shape[0]:
+        if at.numel() != count:
             raise ValueError("one position per row")
-        self._write(0, at, x.shape[0], x, ld)
+        self._write(0, at, count, x, ld, kind)
 
     def _positions(self, rows):
-        if _is_torch_cuda(rows):
-            if rows.dtype != torch.int64 or rows.device.index != self.device:
+        if isinstance(rows, torch.Tensor) and rows.is_cuda:
+            if rows.dtype != torch.int64 or rows.get_device() != self.device:
                 raise ValueError("positions must be an int64 tensor on the index's device")
-            return rows.reshape(-1).contiguous()
+            return rows if rows.dim() == 1 and rows.is_contiguous() else rows.reshape(-1).contiguous()
         return torch.from_numpy(np.ascontiguousarray(rows, dtype=np.int64).reshape(-1)).to(self._dev)
 
-    def _write(self, first, at, count, x, ld):
+    def _write(self, first, at, count, x, ld, kind):
         if count == 0 or self._n == 0:
             return
         check(lib.rag_mx4_write_device(self._st_ref, first, None if at is None else at.data_ptr(),
-                                       None if at is None else self._owner.data_ptr(), count, x.data_ptr(), _type_of(x.dtype), ld,
+                                       None if at is None else self._owner.data_ptr(), count, x.data_ptr(), kind, ld,
                                        self._normalize, self._kept.stream()))
 
     @classmethod
@@ -279,16 +283,18 @@ class QuantizedIndex:
     def reconstruct(self, rows, dtype=None):
         """The values that rows stand for.  Numpy positions: numpy float32, every position inside the index.  CUDA int64
         positions: a CUDA tensor of ``dtype`` (default float32); a position outside the index -- an unfilled slot of a search -- gives zeros."""
-        on_device = _is_torch_cuda(rows)
+        on_device = isinstance(rows, torch.Tensor) and rows.is_cuda
         if not on_device:
             rows = np.ascontiguousarray(rows, dtype=np.int64).reshape(-1)
             if rows.size and (rows.min() < 0 or rows.max() >= self._n):
                 raise ValueError("row position out of range")
         at = self._positions(rows)
-        out = torch.empty((at.numel(), self.dim), dtype=torch.float32 if dtype is None or not on_device else dtype, device=self._dev)
-        kind = _type_of(out.dtype)
-        if at.numel():
-            check(lib.rag_mx4_read_device(self._st_ref, at.data_ptr(), at.numel(), out.data_ptr(), kind, self._kept.stream()))
+        if dtype is None or not on_device:
+            dtype = torch.float32
+        kind, count = _type_of(dtype), at.numel()
+        out = torch.empty((count, self.dim), dtype=dtype, device=self._dev)
+        if count:
+            check(lib.rag_mx4_read_device(self._st_ref, at.data_ptr(), count, out.data_ptr(), kind, self._kept.stream()))
         return out if on_device else out.cpu().numpy()
 
     # ------------------------------------------------------------------ products
@@ -299,11 +305,11 @@ class QuantizedIndex:
         begin = int(begin)
         if not 0 <= begin <= end <= self._n:
             raise ValueError("rows [begin, end) do not lie inside the index")
-        on_device = _is_torch_cuda(q)
-        q, ld = self._rows_in(q, "queries")
-        out = torch.empty((q.shape[0], end - begin), dtype=torch.float32, device=self._dev)
-        if out.numel():
-            check(lib.rag_mx4_scores_device(self._st_ref, begin, end, q.shape[0], q.data_ptr(), _type_of(q.dtype), ld,
+        on_device = isinstance(q, torch.Tensor) and q.is_cuda
+        q, nq, ld, kind = self._rows_in(q, "queries")
+        out = torch.empty((nq, end - begin), dtype=torch.float32, device=self._dev)
+        if nq and end > begin:
+            check(lib.rag_mx4_scores_device(self._st_ref, begin, end, nq, q.data_ptr(), kind, ld,
                                             self._normalize, out.data_ptr(), end - begin, self._kept.stream()))
         return out if on_device else out.cpu().numpy()
 
@@ -315,14 +321,14 @@ class QuantizedIndex:
     def scores_grouped(self, q, groups):
         """Ragged groups in one launch: the scores of each group, [its queries][its rows], one behind the other in a
         flat float32 CUDA tensor.  ``groups``: a ``GroupPlan`` (whose ``split`` gives the views), or what ``plan_groups`` takes."""
-        q, ld = self._rows_in(q, "queries")
-        plan = groups if isinstance(groups, GroupPlan) else self.plan_groups(groups, q.shape[0], q.dtype)
-        if plan.device != self.device or plan.nq != q.shape[0] or plan.type != _type_of(q.dtype) or plan.n > self._n:
+        q, nq, ld, kind = self._rows_in(q, "queries")
+        plan = groups if isinstance(groups, GroupPlan) else self.plan_groups(groups, nq, q.dtype)
+        if plan.device != self.device or plan.nq != nq or plan.type != kind or plan.n > self._n or plan.dim != self.dim:
             raise ValueError("the plan was made for other queries, another device or a longer index")
         out = torch.empty((plan.total,), dtype=torch.float32, device=self._dev)
         if plan.n_items:
             plan._kept.stream()
-            check(lib.rag_mx4_scores_grouped_device(self._st_ref, q.shape[0], q.data_ptr(), plan.type, ld, self._normalize,
+            check(lib.rag_mx4_scores_grouped_device(self._st_ref, nq, q.data_ptr(), plan.type, ld, self._normalize,
                                                     plan.items.data_ptr(), plan.n_items, plan.widest, out.data_ptr(),
                                                     self._kept.stream()))
         return out
@@ -346,14 +352,13 @@ class QuantizedIndex:
             m_ptr = keep.data_ptr()
         else:
             m_ptr = keep = None
-        q, ld = self._rows_in(q, "queries")
-        nq = q.shape[0]
+        q, nq, ld, kind = self._rows_in(q, "queries")
         D = torch.empty((nq, k), dtype=torch.float32, device=dev)
         I = torch.empty((nq, k), dtype=torch.int64, device=dev)
         if nq:
             need = int(lib.rag_mx4_search_workspace(self._n, nq, k))
             ws = torch.empty((need,), dtype=torch.uint8, device=dev)
-            check(lib.rag_mx4_search_device(self._st_ref, nq, q.data_ptr(), _type_of(q.dtype), ld, self._normalize, k,
+            check(lib.rag_mx4_search_device(self._st_ref, nq, q.data_ptr(), kind, ld, self._normalize, k,
                                             -FLT_MAX if min_score is None else float(min_score), m_ptr,
                                             None if self._active is None else self._active.data_ptr(), D.data_ptr(), I.data_ptr(),
                                             ws.data_ptr(), need, self._kept.stream()))

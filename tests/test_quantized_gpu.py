@@ -154,6 +154,42 @@ def test_rows_read_back(n, dim, dtype):
     assert np.array_equal(index.reconstruct(inside), v[inside].astype(np.float32))
 
 
+@pytest.mark.parametrize("dim", [1, 7, 8, 9, 16, 17])
+def test_many_short_rows(dim):
+    """Rows of one or two units of eight elements, many to a workgroup."""
+    import torch
+    from rag_amd import QuantizedIndex
+    rng = np.random.default_rng(dim)
+    n = 70_000
+    x, x64 = _rows(rng, n, dim)
+    index = QuantizedIndex(dim, metric="ip")
+    index.add(x)
+    want = mx4.quantise(x64)
+    _same_packed(index, want)
+    v = mx4.values(*want, dim)
+    at = rng.permutation(n)
+    for name in TYPES:
+        got = index.reconstruct(torch.from_numpy(at).cuda(), dtype=_t(name))
+        assert torch.equal(got.cpu(), torch.from_numpy(v[at]).to(_t(name)))
+
+
+@pytest.mark.parametrize("count", [2, 3, 255, 256, 257, 300])
+def test_repeated_positions_in_short_and_long_writes(count):
+    """Up to 256 positions a workgroup finds repeated ones itself, beyond that they are claimed first: one rule."""
+    import torch
+    rng = np.random.default_rng(count)
+    index, _ = _index(rng, 40, 384)
+    codes, scales = (t.cpu().numpy().copy() for t in index.packed())
+    at = rng.integers(-1, 41, count)
+    x, x64 = _rows(rng, count, 384)
+    index.write(torch.from_numpy(at).cuda(), x)
+    new = mx4.quantise(x64)
+    for i, r in enumerate(at):
+        if 0 <= r < 40:
+            codes[r], scales[r] = new[0][i], new[1][i]
+    _same_packed(index, (codes, scales))
+
+
 def test_every_code_under_every_scale_reads_back():
     """All 16 codes with all 256 scale bytes, in the three types (fp16 overflows and underflows with one rounding)."""
     import torch
