@@ -347,6 +347,7 @@ struct Mx4ScoreArgs {
     const Mx4Item* items;
     // dense: rows [row0, row0 + rows) cut into slabs, every slab against blocks of QB queries
     long long row0, rows, slab, slabs, out_ld;
+    long long total;             // grouped: scores in out (and rows = the store's)
     int nq, nqb;
 };
 
@@ -470,6 +471,10 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     if (a.items) {
         const Mx4Item it = a.items[blockIdx.x];
         row0 = it.row0; at = it.at; ld = it.ld; rows = it.rows; q0 = it.q0; nqh = it.nq;
+        // a piece that was not made for this store, these queries or this result is left out
+        if (rows < 1 || row0 < 0 || row0 > a.rows - rows || nqh < 1 || nqh > QB || q0 < 0 || q0 > a.nq - nqh || ld < rows || at < 0 ||
+            at > a.total - (long long)(nqh - 1) * ld - rows)
+            return;
     } else if (a.nqb == 1) {
         row0 = a.row0; at = 0; ld = a.out_ld; rows = (int)a.rows; q0 = 0; nqh = a.nq;
         first = (int)blockIdx.x * NW + wave;
@@ -982,7 +987,7 @@ int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngro
 }
 
 int rag_mx4_scores_grouped_device(const rag_mx4_store_t* st, int64_t nq, const void* q_dev, int q_type, int64_t q_stride, int normalize,
-                                  const void* items_dev, int64_t n_items, int32_t widest, float* out_dev, void* stream) {
+                                  const void* items_dev, int64_t n_items, int32_t widest, float* out_dev, int64_t total, void* stream) {
     if (int rc = mx4_check_queries(st, nq, q_dev, q_type, q_stride)) return rc;
     if (n_items < 0 || n_items > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "n_items out of range");
     if (n_items == 0) return RAG_OK;
@@ -995,6 +1000,8 @@ int rag_mx4_scores_grouped_device(const rag_mx4_store_t* st, int64_t nq, const v
     Mx4ScoreArgs a = mx4_score_args(st, p, q_dev, q_type, q_stride, normalize ? 1 : 0, out_dev);
     a.items = static_cast<const Mx4Item*>(items_dev);
     a.nq = (int)nq;
+    a.rows = st->n;
+    a.total = total;
     return mx4_launch_any(p, a, n_items, st->device, static_cast<hipStream_t>(stream));
 }
 

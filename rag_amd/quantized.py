@@ -54,7 +54,8 @@ class _Kept:
 
 class GroupPlan:
     """Ragged groups of queries and rows, checked and cut into pieces for the device (``rag_mx4_plan_groups``).
-    ``total``: scores of all groups; ``out_begin[g]``: where those of group g start; ``shapes[g]``: (queries, rows)."""
+    ``total``: scores of all groups; ``out_begin[g]``: where those of group g start; ``shapes[g]``: (queries, rows).
+    Made outside of a graph capture; a graph that uses a plan needs it for as long as it is replayed."""
 
     def __init__(self, groups, nq: int, n: int, dim: int, dtype, device: int):
         g = np.ascontiguousarray(groups, dtype=np.int64)
@@ -62,25 +63,29 @@ class GroupPlan:
             g = g.reshape(0, 4)
         if g.ndim != 2 or g.shape[1] != 4:
             raise ValueError("groups must be [n, 4]: query begin, query end, row begin, row end")
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("groups are planned outside of a graph capture: pass a GroupPlan")
         self.nq, self.n, self.dim, self.type, self.device = int(nq), int(n), int(dim), _type_of(dtype), int(device)
-        self.shapes = np.stack([g[:, 1] - g[:, 0], g[:, 3] - g[:, 2]], 1)
-        self.out_begin = np.zeros(g.shape[0], dtype=np.int64)
+        self._groups = g = g.copy() if g is groups else g
+        self.out_begin = np.empty(g.shape[0], dtype=np.int64)
         count, total, widest = C.c_int64(0), C.c_int64(0), C.c_int32(0)
-
-        def plan(room, ptr):
-            check(lib.rag_mx4_plan_groups(int(dim), self.type, self.nq, self.n, g.shape[0], _ptr(g), room, ptr, C.byref(count),
-                                          _ptr(self.out_begin), C.byref(total), C.byref(widest)))
-        room = 4 * g.shape[0] + 64
-        staging = torch.empty((room, _lib.MX4_ITEM_BYTES), dtype=torch.uint8, pin_memory=True)
-        plan(room, C.c_void_p(staging.data_ptr()))
-        if count.value > room:
-            room = count.value
+        room = 2 * g.shape[0] + 64
+        while True:
             staging = torch.empty((room, _lib.MX4_ITEM_BYTES), dtype=torch.uint8, pin_memory=True)
-            plan(room, C.c_void_p(staging.data_ptr()))
-        self.total, self.widest, self.n_items = int(total.value), int(widest.value), int(count.value)
+            check(lib.rag_mx4_plan_groups(self.dim, self.type, self.nq, self.n, g.shape[0], g.ctypes.data, room, staging.data_ptr(),
+                                          C.byref(count), self.out_begin.ctypes.data, C.byref(total), C.byref(widest)))
+            if count.value <= room:
+                break
+            room = count.value
+        self.total, self.widest, self.n_items = total.value, widest.value, count.value
         self._kept = _Kept(self.device)
         self.items = staging[:self.n_items].to(torch.device("cuda", self.device), non_blocking=True)
         self._kept.tensors = [self.items]
+
+    @property
+    def shapes(self):
+        g = self._groups
+        return np.stack([g[:, 1] - g[:, 0], g[:, 3] - g[:, 2]], 1)
 
     def split(self, scores):
         """The flat result of ``scores_grouped`` as one [queries, rows] view per group."""
@@ -329,7 +334,7 @@ class QuantizedIndex:
         if plan.n_items:
             plan._kept.stream()
             check(lib.rag_mx4_scores_grouped_device(self._st_ref, nq, q.data_ptr(), plan.type, ld, self._normalize,
-                                                    plan.items.data_ptr(), plan.n_items, plan.widest, out.data_ptr(),
+                                                    plan.items.data_ptr(), plan.n_items, plan.widest, out.data_ptr(), plan.total,
                                                     self._kept.stream()))
         return out
 

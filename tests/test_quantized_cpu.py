@@ -91,7 +91,7 @@ def test_arguments_are_refused_before_a_device_is_touched():
         assert lib.rag_mx4_scores_device(s, 0, 10, 1, p, 0, 384, 0, p, 10, None) == bad
         assert lib.rag_mx4_read_device(s, p, 1, p, 0, None) == bad
         assert lib.rag_mx4_write_device(s, 0, None, None, 1, p, 0, 384, 0, None) == bad
-        assert lib.rag_mx4_scores_grouped_device(s, 1, p, 0, 384, 0, p, 1, 1, p, None) == bad
+        assert lib.rag_mx4_scores_grouped_device(s, 1, p, 0, 384, 0, p, 1, 1, p, 100, None) == bad
         assert lib.rag_mx4_search_device(s, 1, p, 0, 384, 0, 10, 0.0, None, None, p, p, p, 1 << 40, None) == bad
     for args in ((-1, 10, 1, p, 0, 384, 0, p, 10), (5, 4, 1, p, 0, 384, 0, p, 10), (0, 101, 1, p, 0, 384, 0, p, 101), (0, 10, -1, p, 0, 384, 0, p, 10),
                  (0, 10, 1, None, 0, 384, 0, p, 10), (0, 10, 1, p, 3, 384, 0, p, 10), (0, 10, 1, p, 0, 383, 0, p, 10), (0, 10, 1, p, 0, 384, 0, None, 10),
@@ -105,7 +105,7 @@ def test_arguments_are_refused_before_a_device_is_touched():
         assert lib.rag_mx4_read_device(ref, *args, None) == bad, args
     for args in ((1, p, 0, 384, 0, p, -1, 1, p), (1, p, 0, 384, 0, None, 1, 1, p), (1, p, 0, 384, 0, p, 1, 1, None), (1, p, 0, 384, 0, p + 8, 1, 1, p),
                  (1, p, 0, 384, 0, p, 1, 0, p), (1, p, 0, 384, 0, p, 1, 2, p), (0, p, 0, 384, 0, p, 1, 1, p)):
-        assert lib.rag_mx4_scores_grouped_device(ref, *args, None) == bad, args
+        assert lib.rag_mx4_scores_grouped_device(ref, *args, 100, None) == bad, args
     for args in ((1, p, 0, 384, 0, 0, 0.0, None, None, p, p), (1, p, 0, 384, 0, 1025, 0.0, None, None, p, p),
                  (1, p, 0, 384, 0, 10, float("nan"), None, None, p, p), (1, p, 0, 384, 0, 10, 0.0, None, None, None, p)):
         assert lib.rag_mx4_search_device(ref, *args, p, 1 << 40, None) == bad, args
@@ -114,7 +114,7 @@ def test_arguments_are_refused_before_a_device_is_touched():
     assert lib.rag_mx4_scores_device(ref, 0, 100, 0, None, 0, 0, 0, None, 100, None) == 0
     assert lib.rag_mx4_write_device(ref, 100, None, None, 0, None, 0, 384, 0, None) == 0
     assert lib.rag_mx4_read_device(ref, None, 0, None, 0, None) == 0
-    assert lib.rag_mx4_scores_grouped_device(ref, 1, p, 0, 384, 0, None, 0, 0, None, None) == 0
+    assert lib.rag_mx4_scores_grouped_device(ref, 1, p, 0, 384, 0, None, 0, 0, None, 0, None) == 0
     assert lib.rag_mx4_search_workspace(100, 1, 0) == -1 and lib.rag_mx4_search_workspace(-1, 1, 1) == -1
     assert lib.rag_mx4_search_workspace(100, 1, 10) > 0
 

@@ -361,6 +361,49 @@ def test_grouped_scores(ngroups, most_q, most_r, dim, nq, dtype):
     _check_scores(full, q64, v, dtype)
 
 
+def test_pieces_that_do_not_fit_are_left_out():
+    """Through the C entry point: pieces for other sizes write nothing, the others their scores."""
+    import ctypes as C
+    import torch
+    from rag_amd import _lib
+    rng = np.random.default_rng(21)
+    index, _ = _index(rng, 200, 64)
+    q, _ = _rows(rng, 3, 64)
+    want = index.scores(q).cpu().numpy()
+    item = np.dtype([("row0", "<i8"), ("at", "<i8"), ("rows", "<i4"), ("ld", "<i4"), ("q0", "<i4"), ("nq", "<i4")])
+    good = [(0, 0, 50, 50, 0, 3), (150, 150, 50, 60, 1, 2)]
+    bad = [(151, 0, 50, 50, 0, 1), (-1, 0, 5, 5, 0, 1), (0, 0, 0, 5, 0, 1), (0, -1, 5, 5, 0, 1), (0, 0, 5, 4, 0, 1), (0, 0, 5, 5, 1, 3),
+           (0, 0, 5, 5, -1, 1), (0, 0, 5, 5, 0, 4), (0, 0, 5, 5, 0, 0), (0, 256, 5, 5, 0, 1), (0, 100, 50, 60, 0, 3), (2 ** 62, 0, 5, 5, 0, 1),
+           (0, 2 ** 62, 5, 5, 0, 1)]
+    items = torch.from_numpy(np.array(bad[:6] + good + bad[6:], dtype=item).view(np.uint8)).cuda()
+    out = torch.full((260,), 7.0, device="cuda")
+    _lib.check(_lib.lib.rag_mx4_scores_grouped_device(C.byref(index._st), 3, q.data_ptr(), 0, 64, 0, items.data_ptr(), len(good) + len(bad), 3,
+                                                      out.data_ptr(), 260, torch.cuda.current_stream().cuda_stream))
+    got = out.cpu().numpy()
+    expect = np.full(260, 7.0, np.float32)
+    expect[:150] = want[:, :50].reshape(-1)
+    expect[150:200], expect[210:260] = want[1, 150:], want[2, 150:]
+    assert np.array_equal(got, expect)
+
+
+def test_groups_are_planned_outside_of_a_capture():
+    import torch
+    rng = np.random.default_rng(22)
+    index, _ = _index(rng, 64, 64)
+    q, _ = _rows(rng, 2, 64)
+    graph = torch.cuda.CUDAGraph()
+    said = None
+    with torch.cuda.graph(graph):
+        out = index.scores(q)
+        try:
+            index.scores_grouped(q, [[0, 2, 0, 64]])
+        except ValueError as e:
+            said = str(e)
+    assert "outside of a graph capture" in said
+    graph.replay()
+    assert torch.equal(out, index.scores(q))
+
+
 def test_groups_that_leave_nothing():
     import torch
     rng = np.random.default_rng(8)
