@@ -27,7 +27,9 @@ class SearchConfig:
     search here is exact (or IVF when asked).  A ``quantization_config`` (the reference hands
     it to the collection, :130, where the server searches a compressed copy and re-scores with
     the originals) switches on the device-side equivalent: a bf16 copy of the rows searched
-    first, the kept rows re-scored in fp32 -- answers unchanged."""
+    first, the kept rows re-scored in fp32 -- answers unchanged.  With the key ``"mx4"`` in it
+    the rows are kept at four bits only (``rag_amd.QuantizedIndex``, 0.53 bytes per element,
+    flat COSINE and DOT_PRODUCT collections): the answers are exact for the rows as stored."""
     dimension: int
     metric: MetricType = MetricType.COSINE
     collection_name: str = "default"

@@ -27,6 +27,10 @@ from .schemas import Chunk, IndexType, MetricType, SearchConfig, SearchError, de
 _METRIC = {MetricType.COSINE: "cosine", MetricType.DOT_PRODUCT: "ip", MetricType.EUCLIDEAN: "l2"}
 
 
+def _four_bit(config: SearchConfig) -> bool:
+    return config.quantization_config is not None and "mx4" in config.quantization_config
+
+
 class HipSearchOptimizer:
     def __init__(self, config: SearchConfig, qdrant_client=None):
         # `qdrant_client` is accepted for signature compatibility (search_optimizer.py:76) and unused
@@ -39,9 +43,15 @@ class HipSearchOptimizer:
         kind = "ivf" if config.index_type == IndexType.IVF else "flat"
         if config.metric == MetricType.EUCLIDEAN and kind != "flat":
             raise SearchError("the euclidean metric needs a flat index on the HIP backend")
-        self.index = DeviceIndex(config.dimension, metric=_METRIC[config.metric], kind=kind, device=config.device)
-        if config.quantization_config is not None and kind == "flat" and config.metric != MetricType.EUCLIDEAN:
-            self.index.set_prefilter(True)
+        if _four_bit(config):
+            if kind != "flat" or config.metric == MetricType.EUCLIDEAN:
+                raise SearchError("four-bit rows need a flat index with the cosine or dot metric on the HIP backend")
+            from .quantized import QuantizedIndex
+            self.index = QuantizedIndex(config.dimension, metric=_METRIC[config.metric], device=config.device)
+        else:
+            self.index = DeviceIndex(config.dimension, metric=_METRIC[config.metric], kind=kind, device=config.device)
+            if config.quantization_config is not None and kind == "flat" and config.metric != MetricType.EUCLIDEAN:
+                self.index.set_prefilter(True)
         self.payloads: List[Dict[str, Any]] = []       # row position -> payload
         self.point_ids: List[Any] = []                 # row position -> point id given at upsert
         self._row_of: Dict[Any, int] = {}              # point id -> live row position
@@ -110,7 +120,7 @@ class HipSearchOptimizer:
             return hit[1]
         mask = np.fromiter((payload_passes(p, filters) for p in self.payloads), dtype=np.uint8,
                            count=len(self.payloads))
-        if isinstance(self.index, DeviceIndex) and len(self.index) == mask.size:
+        if (isinstance(self.index, DeviceIndex) or _four_bit(self.config)) and len(self.index) == mask.size:
             # the bytes stay on the device beside the rows (the server's payload index in the reference): a
             # repeated filter is not uploaded again
             mask = self.index.make_filter(mask)
@@ -205,7 +215,11 @@ class HipSearchOptimizer:
         self.client = None
         self.collection_name = config.collection_name
         self.logger = logging.getLogger(__name__)
-        self.index = DeviceIndex.load(path, device=config.device)
+        if _four_bit(config):
+            from .quantized import QuantizedIndex
+            self.index = QuantizedIndex.load(path, device=config.device)
+        else:
+            self.index = DeviceIndex.load(path, device=config.device)
         self.payloads = meta["payloads"]
         self.point_ids = meta["point_ids"]
         self._row_of = {self.point_ids[r]: r for r in meta["live_rows"]}

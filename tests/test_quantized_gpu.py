@@ -571,6 +571,47 @@ def test_snapshot_round_trip(tmp_path):
         assert np.array_equal(a, b)
 
 
+def test_optimizer_over_four_bit_rows(tmp_path):
+    """SearchConfig(quantization_config={"mx4": ...}): upsert, search, filters, soft delete, vectors and backup of a collection."""
+    from rag_amd.schemas import IndexType, MetricType, SearchConfig, SearchError
+    from rag_amd.search_optimizer import HipSearchOptimizer
+    rng = np.random.default_rng(14)
+    n, dim = 3000, 96
+    x = rng.standard_normal((n, dim)).astype(np.float32)
+    config = SearchConfig(dimension=dim, metric=MetricType.COSINE, collection_name="c", quantization_config={"mx4": {}})
+    opt = HipSearchOptimizer(config)
+    meta = [{"chunk_id": f"c{i}", "document_id": 1, "page": i % 5, "text": str(i)} for i in range(n)]
+    opt.upsert(x, meta, list(range(n)))
+    opt.upsert(x[:1] * -1, [dict(meta[7])], [7])                     # point 7 is replaced
+    codes, scales = opt.index.packed()
+    v = mx4.values(codes.cpu().numpy(), scales.cpu().numpy(), dim)
+    q = rng.standard_normal((4, dim)).astype(np.float32)
+    s = mx4.scores(q / np.linalg.norm(q.astype(np.float64), axis=1, keepdims=True), v)
+    s[:, 7] = -np.inf
+
+    def check(lists, allowed=None, limit=10):
+        for i, hits in enumerate(lists):
+            order = np.argsort(-(s[i] if allowed is None else np.where(allowed, s[i], -np.inf)))[:limit]
+            assert [h[0].metadata["text"] for h in hits] == [str(r) if r < n else "7" for r in order]
+            assert np.allclose([h[1] for h in hits], s[i][order], rtol=1e-6, atol=1e-7)
+    check(opt.batch_search_sync(q, limit=10, min_score=-1.0))
+    assert opt.index.last_path == "mx4"
+    check([opt.search_sync(q[0].tolist(), limit=3, min_score=-1.0)], limit=3)
+    pages = np.array([i % 5 == 2 for i in range(n)] + [True])
+    for _ in range(2):                                               # the second time with the filter kept on the device
+        check(opt.batch_search_sync(q, limit=10, min_score=-1.0, filters={"page": 2}), pages)
+    assert opt.get_vector(5)["vector"] == v[5].astype(np.float32).tolist()
+    path = str(tmp_path / "c.bin")
+    opt.backup(path)
+    again = HipSearchOptimizer.restore(path, config)
+    check(again.batch_search_sync(q, limit=10, min_score=-1.0))
+    opt.set_points_active(False)
+    assert opt.search_sync(q[0].tolist(), limit=3, min_score=-1.0) == []
+    for kwargs in ({"metric": MetricType.EUCLIDEAN}, {"index_type": IndexType.IVF}):
+        with pytest.raises(SearchError):
+            HipSearchOptimizer(SearchConfig(dimension=dim, collection_name="c", quantization_config={"mx4": {}}, **kwargs))
+
+
 def test_refusals():
     import torch
     from rag_amd import QuantizedIndex, RagHipError
