@@ -438,6 +438,17 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long lo
     __syncthreads();
 }
 
+// four values over four columns of lanes, transposed: column c of v_s goes to column s of v_c
+__device__ __forceinline__ void columns_transpose(float* v) {
+    const v2u a = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(v[0]), __float_as_uint(v[2]), false, false));
+    const v2u b = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(v[1]), __float_as_uint(v[3]), false, false));
+    const v2u c = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false));
+    const v2u d = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false));
+    v[0] = __uint_as_float(c.x);
+    v[1] = __uint_as_float(c.y);
+    v[2] = __uint_as_float(d.x);
+    v[3] = __uint_as_float(d.y);
+}
 // lanes of column s (0, 1, 2) receive v_s of column 3
 __device__ __forceinline__ float fifth_digits(float v0, float v1, float v2) {
     const v2u a = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(v0), __float_as_uint(v2), false, false));
@@ -447,24 +458,37 @@ __device__ __forceinline__ float fifth_digits(float v0, float v1, float v2) {
     return __uint_as_float(r.y);                                // the odd columns of both in turn: v0, v1, v2, v1 of column 3
 }
 
-// ND digits, MT tiles of queries, NB blocks of 16 rows per wave, U blocks of 128 along the row fetched together, NW waves;
-// ONE: U blocks are the whole row.
+// ND digits, MT tiles of queries, NB blocks of 16 rows per wave, U blocks of 128 along the row fetched together, NW waves.
+// STEPS 1 or 2: that many fetches are a row; 0: as many as it takes.
 //
 // A wave takes 16 NB rows at a time and keeps the next U blocks of them in flight while the present ones go through the
-// matrix unit; nothing but the query fragments goes through LDS, and there is no barrier after they are staged.  The fetch
-// ahead is unconditional (past the last rows it repeats them): behind a branch the compiler would wait for it at once.
-template <int ND, int MT, int NB, int U, int NW, bool ONE, bool NT>
+// matrix unit; nothing but the query fragments goes through LDS, and there is no barrier after they are staged.  The wave's
+// memory operations are the same whatever the data: the fetch ahead is made past the last rows too (of the last ones again), and
+// lanes without a score to store address nothing behind a buffer descriptor's end.  Behind a branch the compiler would have to
+// wait for all of them at every turn, stores too (256 fp32 queries x 200k x 768: 160 us with branches around the stores, 156 without).
+//
+// BIG, for stores larger than the caches: rows are fetched past them (4M x 768, one query: 299 -> 264 us), and where up to 8
+// queries meet a row a wave takes four tiles of sixteen rows in a row and stores their scores together, 256 contiguous bytes
+// per query instead of 64 (264 -> 255).
+//
+// Where it stands.  Few queries: bound by HBM.  4M x 768, one query: 255 us, 6.6 TB/s of rows, scales and scores; reading the same
+// rows alone takes 220 us (7.0 TB/s), and with one 256-byte store per 24 KB 236 to 247.  16 bf16 queries x 1M x 1024: 113 us, 5.4 TB/s
+// (100 without the stores).  Many queries: bound by the matrix unit and the LDS that feeds it (a tile's fragments serve NB row blocks):
+// 256 fp32 queries x 200k x 768: 156 us, 2.5e15 eight-bit operations a second, against 2.8e15 of a large library product of eight-bit matrices.
+template <int ND, int MT, int NB, int U, int NW, int STEPS, bool BIG>
 __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     typedef Mx4Digits<ND, MT> L;
     constexpr int QPT = L::QPT, TILES = L::TILES, QB = MT * QPT;
-    constexpr int SW = (U + 3) / 4;                             // scale dwords per fetch
-    const int ks = ONE ? U : a.ks, ksu = ONE ? U : a.ksu;
+    constexpr bool LONG = BIG && MT <= 2;
+    static_assert(!LONG || NB == 1, "four tiles of one row block each are stored together");
+    const int ks = STEPS ? STEPS * U : a.ks, ksu = STEPS ? STEPS * U : a.ksu;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     uint8_t* frag = smem;
     uint8_t* sc = frag + (size_t)ksu * TILES * 2048;
     float* inv = reinterpret_cast<float*>(sc + (size_t)((ksu + 3) / 4) * TILES * 256);
 
     // rows [row0, row0 + rows) against queries [q0, q0 + nqh); this wave takes the tiles of 16 NB rows first, first + stride, ...
+    // (LONG: four from each)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     long long row0, at, ld;
     int rows, q0, nqh, first = wave, stride = NW;
@@ -494,11 +518,14 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         at = (long long)q0 * a.out_ld + lo;
         ld = a.out_ld;
     }
+    if (LONG) first *= 4;
     const int n16 = lane & 15, col = lane >> 4;
     const int tiles = rows / (16 * NB) + (rows % (16 * NB) != 0);
+    const int end = LONG ? (tiles + 3) & ~3 : tiles;
     const int sd = (ks + 3) / 4;                                // scale dwords of a lane per row
     float* out = a.out + at;
 
+    constexpr int SW = (U + 3) / 4 + (STEPS == 2 && U % 4 ? 1 : 0);     // scale dwords per fetch
     struct Buf {
         v4i w[NB][U];
         int s[NB][SW];
@@ -508,8 +535,10 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     // uniform part, a block or scale dword of the tile's first row, always lies inside the store.)
     const int l0 = (int)(row0 & 15) + n16;                      // tiles start at multiples of 16 from row0
     const int wo = (l0 >> 4) * 16 * a.code_ld + (l0 & 15) * 64 + col * 16, so = n16 * a.scale_ld + col * 4;
-    constexpr int AUX = NT ? 2 : 0;                             // 2: not to be kept in the caches
-    auto load = [&](Buf& b, int tile, int ks0) {
+    constexpr int AUX = BIG ? 2 : 0;                            // 2: not to be kept in the caches
+    auto load = [&](Buf& b, int tile, auto ks0c) {              // ks0c: a constant where STEPS is 1 or 2
+        const int ks0 = ks0c;
+        tile = tile < tiles ? tile : tiles - 1;
         const long long r0 = row0 + (long long)tile * (16 * NB);
         const size_t wat = (size_t)(r0 >> 4) * 16 * a.code_ld, sat = (size_t)r0 * a.scale_ld;
         const size_t wleft = a.code_bytes - wat, sleft = a.scale_bytes - sat;
@@ -519,22 +548,24 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int k = ONE ? u : ks0 + u < ks ? ks0 + u : ks - 1;      // blocks past the row's meet zero digits
+                const int k = STEPS || ks0 + u < ks ? ks0 + u : ks - 1;          // blocks past the row's meet zero digits
                 b.w[nb][u] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(wr, wo + nb * 16 * a.code_ld, k * 1024, AUX));
             }
 #pragma unroll
             for (int d = 0; d < SW; ++d) {
-                const int k = ONE ? d : (ks0 >> 2) + d < sd ? (ks0 >> 2) + d : sd - 1;
+                const int k = (ks0 >> 2) + d < sd ? (ks0 >> 2) + d : sd - 1;
                 b.s[nb][d] = (int)__builtin_amdgcn_raw_buffer_load_b32(sr, so + nb * 16 * a.scale_ld, k * 16, 0);
             }
         }
     };
     v4f acc[TILES][NB];
-    auto multiply = [&](const Buf& b, int ks0, auto first_of_row) {
+    auto multiply = [&](const Buf& b, auto ks0c, auto first_of_row) {
+        const int ks0 = ks0c;
         constexpr bool FIRST = decltype(first_of_row)::value;   // begins the sums at zero
-        constexpr bool SHIFT = !ONE && U < 4;                   // the fetch may begin inside a scale dword
+        constexpr bool SHIFT = STEPS == 0 && U < 4;             // the fetch may begin inside a scale dword
+        constexpr int K0 = [] { if constexpr (STEPS) return decltype(ks0c)::value; else return 0; }();
         const uint8_t* f = frag + (size_t)ks0 * TILES * 2048;
-        int fl = (col * 16 + (n16 ^ col)) * 16, sl = lane * 4;     // places of the first half; the second half's differ in bit 2 of the row
+        int fl = (col * 16 + (n16 ^ col)) * 16, sl = lane * 4;  // places of the first half; the second half's differ in bit 2 of the row
         if constexpr (TILES > 1) asm volatile("" : "+v"(fl), "+v"(sl));      // more than one tile's fragments do not fit the registers: read from LDS each time
         // query fragments AHEAD tiles ahead: the LDS latency passes under the products of the tiles before
         constexpr int AHEAD = 2, RING = AHEAD + 1;
@@ -557,6 +588,7 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         });
         static_for<U * TILES>([&](auto ic) {
             constexpr int i = decltype(ic)::value, u = i / TILES, mt = i % TILES;
+            constexpr int kk = K0 + u;                          // (K0 is a multiple of 4, or shifted away, where STEPS is 0)
             if constexpr (i + AHEAD < U * TILES) fetch(std::integral_constant<int, i + AHEAD>{});
             if constexpr (TILES > 1) __builtin_amdgcn_sched_barrier(0);
             const v8i x = __builtin_shufflevector(lo[i % RING], hi[i % RING], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -564,79 +596,152 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
             for (int nb = 0; nb < NB; ++nb) {
                 const v8i y = __builtin_shufflevector(b.w[nb][u], b.w[nb][u], 0, 1, 2, 3, -1, -1, -1, -1);
                 const v4f c = FIRST && u == 0 ? (v4f){0.f, 0.f, 0.f, 0.f} : acc[mt][nb];
-                acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 4, u & 3, xs[i % RING], u & 3, ys[nb][u / 4]);
+                acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 4, kk & 3, xs[i % RING], kk & 3,
+                                                                               ys[nb][(kk >> 2) - (K0 >> 2)]);
             }
         });
     };
     float iv[MT];
-    float* const op = out + col * ld + n16;
-    auto store = [&](int tile) {
+    unsigned place[MT];                                         // of this lane's score from the tile's first one; past the end where there is none
+    constexpr unsigned NOWHERE = 0x80000000u;
+    float held[MT][4];                                          // LONG: the scores of the tiles since the last store
+    auto total = [&](int mt, int nb) -> float {
         // column c of lanes holds query c of the tile; the order of the additions is the same for every query, so a score does
         // not depend on what it is computed together with
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const int r = (tile * NB + nb) * 16;
-            float y[MT];
+        const v4f v = acc[mt][nb];
+        float y = (v[0] + v[1]) + (v[2] + v[3]);
+        if constexpr (L::INSIDE) y += fifth_digits(v[0], v[1], v[2]);
+        else if constexpr (ND == 5) y += acc[MT + mt / 4][nb][mt & 3];
+        y *= iv[mt];
+        if constexpr (STEPS == 0) asm volatile("" : "+v"(y));   // here: else the products sink into the branch that asks whether a row is done
+        return y;
+    };
+    auto put = [&](float v, float* base, int bytes, unsigned offset) {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), __builtin_amdgcn_make_buffer_rsrc(base, 0, bytes, 0x00027000), offset, 0, 0);
+    };
+    auto store = [&](int tile) {
+        if constexpr (LONG) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const v4f v = acc[mt][nb];
-                y[mt] = (v[0] + v[1]) + (v[2] + v[3]);
-                if constexpr (L::INSIDE) y[mt] += fifth_digits(v[0], v[1], v[2]);
-                else if constexpr (ND == 5) y[mt] += acc[MT + mt / 4][nb][mt & 3];
-                y[mt] *= iv[mt];
-                asm volatile("" : "+v"(y[mt]));                 // here: else the products sink into the branches below
-            }
-            if (r + n16 < rows && col < QPT) {
+                columns_transpose(held[mt]);
+                const int r = (tile - 3) * 16, left = (rows - r) * 4 < 256 && rows - r < 64 ? (rows - r) * 4 : 256;
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-                    if (mt * QPT + col < nqh) op[mt * QPT * ld + r] = y[mt];
+                for (int s = 0; s < QPT; ++s)
+                    put(held[mt][s], out + (mt * QPT + s) * ld + r, mt * QPT + s < nqh ? left : 0, lane * 4);
+            }
+        } else {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const int r = (tile * NB + nb) * 16;
+                const bool there = r + n16 < rows;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) put(total(mt, nb), out + mt * QPT * ld + r, 0x7fffffff, there ? place[mt] : NOWHERE);
             }
         }
     };
 
     Buf x, y;
-    int t = first, k = 0;
-    load(x, t < tiles ? t : tiles - 1, 0);                      // on its way while the queries are split
+    typedef std::integral_constant<int, 0> Zero;
+    typedef std::integral_constant<int, U> Half;
+    int t = first;
+    if constexpr (STEPS) load(x, t, Zero{});                    // on its way while the queries are split
+    else load(x, t, 0);
     mx4_stage_queries<ND, MT, NW * 64>(a, q0, nqh, frag, sc, inv);
-    if (first >= tiles) return;
+    if (first >= end) return;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) iv[mt] = inv[col < QPT ? mt * QPT + col : 0];
-    auto piece = [&](const Buf& b, int ks0) {
-        if (ONE || ks0 == 0) multiply(b, ks0, std::true_type{});
-        else multiply(b, ks0, std::false_type{});
+    for (int mt = 0; mt < MT; ++mt) {
+        iv[mt] = inv[col < QPT ? mt * QPT + col : 0];
+        place[mt] = col < QPT && mt * QPT + col < nqh ? (unsigned)(col * ld + n16) * 4u : NOWHERE;
+    }
+    auto hold = [&](auto sub) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) held[mt][decltype(sub)::value] = total(mt, 0);
     };
-    for (;;) {
-        // where the piece behind this one lies, and the one behind that
-        auto next = [&](int& t2, int& k2) {
-            if (!ONE) {
-                k2 += U;
-                if (k2 < ksu) return;
-                k2 = 0;
-            }
-            t2 += stride;
+    if constexpr (STEPS == 1) {
+        // pairs of tiles: x and y in turn (LONG: two pairs to a store)
+        for (;;) {
+            static_for<LONG ? 2 : 1>([&](auto pair) {
+                constexpr int p = decltype(pair)::value * 2;
+                const int t1 = LONG ? t + p + 1 : t + stride;
+                const int t2 = LONG ? (p == 0 ? t + 2 : t + 4 * stride) : t + 2 * stride;
+                load(y, t1, Zero{});
+                __builtin_amdgcn_sched_barrier(0);              // the fetch goes out before the products wait for theirs
+                multiply(x, Zero{}, std::true_type{});
+                if constexpr (LONG) hold(std::integral_constant<int, p>{});
+                else store(t);
+                if (!LONG && t1 >= end) return;
+                load(x, t2, Zero{});
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(y, Zero{}, std::true_type{});
+                if constexpr (LONG) hold(std::integral_constant<int, p + 1>{});
+                else store(t1);
+            });
+            if constexpr (LONG) store(t + 3);
+            t += LONG ? 4 * stride : 2 * stride;
+            if (t >= end) break;
+        }
+    } else if constexpr (STEPS == 2 && !LONG) {
+        for (;;) {
+            load(y, t, Half{});
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(x, Zero{}, std::true_type{});
+            load(x, t + stride, Zero{});
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(y, Half{}, std::false_type{});
+            store(t);
+            t += stride;
+            if (t >= end) break;
+        }
+    } else {
+        int k = 0;
+        auto piece = [&](const Buf& b, int ks0) {
+            if (ks0 == 0) multiply(b, ks0, std::true_type{});
+            else multiply(b, ks0, std::false_type{});
         };
-        int t2 = t, k2 = k;
-        next(t2, k2);
-        load(y, t2 < tiles ? t2 : tiles - 1, k2);
-        __builtin_amdgcn_sched_barrier(0);                      // the fetch goes out before the products wait for theirs
-        piece(x, k);
-        if (k2 == 0) store(t);
-        if (t2 >= tiles) break;
-        t = t2;
-        k = k2;
-        next(t, k);
-        load(x, t < tiles ? t : tiles - 1, k);
-        __builtin_amdgcn_sched_barrier(0);
-        piece(y, k2);
-        if (k == 0) store(t2);
-        if (t >= tiles) break;
+        // where the piece behind this one lies
+        auto next = [&](int& t2, int& k2) {
+            k2 += U;
+            if (k2 < ksu) return;
+            k2 = 0;
+            t2 += !LONG ? stride : (t2 & 3) != 3 ? 1 : 4 * stride - 3;
+        };
+        auto done = [&](int tile) {
+            if constexpr (LONG) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    held[mt][0] = held[mt][1];
+                    held[mt][1] = held[mt][2];
+                    held[mt][2] = held[mt][3];
+                    held[mt][3] = total(mt, 0);
+                }
+                if ((tile & 3) != 3) return;
+            }
+            store(tile);
+        };
+        for (;;) {
+            int t2 = t, k2 = k;
+            next(t2, k2);
+            load(y, t2, k2);
+            __builtin_amdgcn_sched_barrier(0);
+            piece(x, k);
+            if (k2 == 0) done(t);
+            if (t2 >= end) break;
+            t = t2;
+            k = k2;
+            next(t, k);
+            load(x, t, k);
+            __builtin_amdgcn_sched_barrier(0);
+            piece(y, k2);
+            if (k == 0) done(t2);
+            if (t >= end) break;
+        }
     }
 }
 
 // Which kernel a product takes: from the queries that meet a row, and the row's length.
 struct Mx4Shape {
-    int nd, mt, nb, u, nw, ksu, qb;
-    bool one, nt;
+    int nd, mt, nb, u, nw, steps, ksu, qb;
+    bool big;
     size_t lds;
 };
 static int mx4_tiles(int nd, int mt) { return nd == 5 && mt > 1 ? mt + (mt + 3) / 4 : mt; }        // Mx4Digits::TILES
@@ -644,19 +749,24 @@ static size_t mx4_lds(int ks, int u, int tiles) {
     const int ksu = (ks + u - 1) / u * u;
     return (size_t)ksu * tiles * 2048 + (size_t)(ksu + 3) / 4 * tiles * 256 + (size_t)tiles * 4 * sizeof(float);
 }
-static Mx4Shape mx4_shape(int type, int dim, long long nq) {
+// wide: the scores of two queries may lie further apart than a lane's 32-bit offset reaches (LONG kernels have none)
+static Mx4Shape mx4_shape(int type, int dim, long long nq, bool wide) {
     Mx4Shape p = {};
     const int ks = mx4_blocks(dim);
     p.nd = type == RAG_MX4_F32 ? 5 : 4;
-    auto fetch = [&](int mt) {
-        if (mt <= 2) return ks <= 8 ? ks : (ks & 7) == 0 || (ks & 7) > 4 ? 8 : 4;
-        if (mt == 4) return ks == 3 ? 3 : (ks & 3) == 0 ? 4 : (ks & 1) == 0 ? 2 : 1;
-        return (ks & 1) == 0 ? 2 : 1;
+    // rows of up to 8 blocks: one fetch, or two of half the row where more tiles need the registers
+    auto fetch = [&](int mt, int* steps) {
+        *steps = mt <= 2 ? ks <= 8 : ks <= 3 ? 1 : ks == 4 || ks == 6 || ks == 8 ? 2 : 0;
+        if (mt == 8 && ks == 8) *steps = 0;
+        if (*steps) return ks / *steps;
+        if (mt <= 2) return (ks & 7) == 0 || (ks & 7) > 4 ? 8 : 4;
+        return mt == 4 && (ks & 3) == 0 ? 4 : (ks & 1) == 0 ? 2 : 1;
     };
     p.mt = nq <= (p.nd == 5 ? 3 : 4) ? 1 : nq <= 8 ? 2 : nq <= 16 ? 4 : 8;
-    while (p.mt > 1 && mx4_lds(ks, fetch(p.mt), mx4_tiles(p.nd, p.mt)) > 160 * 1024) p.mt /= 2;
-    p.u = fetch(p.mt);
-    p.one = p.mt <= 2 && p.u == ks;
+    if (wide) p.mt = std::min(p.mt, 2);
+    while (p.mt > 1 && mx4_lds(ks, fetch(p.mt, &p.steps), mx4_tiles(p.nd, p.mt)) > 160 * 1024) p.mt /= 2;
+    p.u = fetch(p.mt, &p.steps);
+    p.big = wide;
     p.nb = p.mt <= 4 ? 1 : 2;
     p.nw = p.mt >= 4 ? 8 : 4;
     p.ksu = (ks + p.u - 1) / p.u * p.u;
@@ -664,11 +774,12 @@ static Mx4Shape mx4_shape(int type, int dim, long long nq) {
     p.lds = mx4_lds(ks, p.u, mx4_tiles(p.nd, p.mt));
     return p;
 }
+constexpr long long MX4_WIDE = 100 * 1000 * 1000;        // 3 * 4 bytes * this, and a tile, stay below 2^31
 
-template <int ND, int MT, int NB, int U, int NW, bool ONE, bool NT>
+template <int ND, int MT, int NB, int U, int NW, int STEPS, bool BIG>
 static int mx4_launch(const Mx4ScoreArgs& a, long long grid, size_t lds, int device, hipStream_t s) {
     static bool attr_set[64] = {};          // per device: the attribute belongs to the device's code object
-    auto kern = mx4_scores_kernel<ND, MT, NB, U, NW, ONE, NT>;
+    auto kern = mx4_scores_kernel<ND, MT, NB, U, NW, STEPS, BIG>;
     if (lds > 48 * 1024 && !attr_set[device & 63]) {
         RAG_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         attr_set[device & 63] = true;
@@ -679,15 +790,18 @@ static int mx4_launch(const Mx4ScoreArgs& a, long long grid, size_t lds, int dev
 }
 template <int ND>
 static int mx4_launch_nd(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s) {
-#define MX4_CASE(MT, NB, U, NW, ONE) if (p.mt == MT && p.u == U && p.one == ONE) return p.nt ? mx4_launch<ND, MT, NB, U, NW, ONE, true>(a, grid, p.lds, device, s) : mx4_launch<ND, MT, NB, U, NW, ONE, false>(a, grid, p.lds, device, s)
+#define MX4_CASE(MT, NB, U, NW, STEPS) \
+    if (p.mt == MT && p.u == U && p.steps == STEPS) \
+        return p.big ? mx4_launch<ND, MT, NB, U, NW, STEPS, true>(a, grid, p.lds, device, s) : mx4_launch<ND, MT, NB, U, NW, STEPS, false>(a, grid, p.lds, device, s)
 #define MX4_FEW(MT) \
-    MX4_CASE(MT, 1, 1, 4, true); MX4_CASE(MT, 1, 2, 4, true); MX4_CASE(MT, 1, 3, 4, true); MX4_CASE(MT, 1, 4, 4, true); \
-    MX4_CASE(MT, 1, 5, 4, true); MX4_CASE(MT, 1, 6, 4, true); MX4_CASE(MT, 1, 7, 4, true); MX4_CASE(MT, 1, 8, 4, true); \
-    MX4_CASE(MT, 1, 4, 4, false); MX4_CASE(MT, 1, 8, 4, false)
+    MX4_CASE(MT, 1, 1, 4, 1); MX4_CASE(MT, 1, 2, 4, 1); MX4_CASE(MT, 1, 3, 4, 1); MX4_CASE(MT, 1, 4, 4, 1); MX4_CASE(MT, 1, 5, 4, 1); \
+    MX4_CASE(MT, 1, 6, 4, 1); MX4_CASE(MT, 1, 7, 4, 1); MX4_CASE(MT, 1, 8, 4, 1); MX4_CASE(MT, 1, 4, 4, 0); MX4_CASE(MT, 1, 8, 4, 0)
     MX4_FEW(1);
     MX4_FEW(2);
-    MX4_CASE(4, 1, 1, 8, false); MX4_CASE(4, 1, 2, 8, false); MX4_CASE(4, 1, 3, 8, false); MX4_CASE(4, 1, 4, 8, false);
-    MX4_CASE(8, 2, 1, 8, false); MX4_CASE(8, 2, 2, 8, false);
+    MX4_CASE(4, 1, 1, 8, 1); MX4_CASE(4, 1, 2, 8, 1); MX4_CASE(4, 1, 3, 8, 1); MX4_CASE(4, 1, 2, 8, 2); MX4_CASE(4, 1, 3, 8, 2); MX4_CASE(4, 1, 4, 8, 2);
+    MX4_CASE(4, 1, 1, 8, 0); MX4_CASE(4, 1, 2, 8, 0); MX4_CASE(4, 1, 4, 8, 0);
+    MX4_CASE(8, 2, 1, 8, 1); MX4_CASE(8, 2, 2, 8, 1); MX4_CASE(8, 2, 3, 8, 1); MX4_CASE(8, 2, 2, 8, 2); MX4_CASE(8, 2, 3, 8, 2);
+    MX4_CASE(8, 2, 1, 8, 0); MX4_CASE(8, 2, 2, 8, 0);
 #undef MX4_FEW
 #undef MX4_CASE
     return fail(RAG_ERR_INVALID, "internal: no four-bit product kernel for this shape");
@@ -742,9 +856,9 @@ static Mx4ScoreArgs mx4_score_args(const rag_mx4_store_t* st, const Mx4Shape& p,
 // scores of rows [row0, row0 + rows) (checked by the caller)
 static int mx4_scores(const rag_mx4_store_t* st, long long row0, long long rows, long long nq, const void* q, int q_type, long long ldq,
                       int normalize, float* out, long long out_ld, hipStream_t s) {
-    Mx4Shape p = mx4_shape(q_type, st->dim, nq);
+    Mx4Shape p = mx4_shape(q_type, st->dim, nq, out_ld > MX4_WIDE);
     Mx4ScoreArgs a = mx4_score_args(st, p, q, q_type, ldq, normalize, out);
-    p.nt = nq <= p.qb && rows * a.code_ld > (getenv("MXNT") ? atoll(getenv("MXNT")) << 20 : 64LL << 20);
+    p.big = p.big || (nq <= p.qb && rows * a.code_ld > 64LL << 20);
     a.row0 = row0;
     a.rows = rows;
     a.out_ld = out_ld;
@@ -752,7 +866,7 @@ static int mx4_scores(const rag_mx4_store_t* st, long long row0, long long rows,
     a.nqb = (int)((nq + p.qb - 1) / p.qb);
     const long long unit = 16LL * p.nb * p.nw;                  // rows of one step of a workgroup
     const long long units = (rows + unit - 1) / unit;
-    if (a.nqb == 1) return mx4_launch_any(p, a, std::min<long long>(units, getenv("MXG") ? atoi(getenv("MXG")) : p.mt == 8 ? 256 : p.mt == 4 ? 512 : 1024), st->device, s);
+    if (a.nqb == 1) return mx4_launch_any(p, a, std::min<long long>(units, p.mt == 8 ? 256 : p.mt == 4 ? 512 : 1024), st->device, s);
     // Slabs: as many as make the workgroups come out even over the chip's compute units, each long against the staging of
     // its queries (about two units of work)
     const long long seats = 256LL * (p.mt == 8 ? 1 : 2);
@@ -955,7 +1069,7 @@ int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngro
     }
     *total = sum;
     *widest = (int32_t)most_q;
-    const Mx4Shape p = mx4_shape(q_type, dim, std::max<long long>(most_q, 1));
+    const Mx4Shape p = mx4_shape(q_type, dim, std::max<long long>(most_q, 1), sum > MX4_WIDE);       // (no group has more rows than scores)
     // rows of an item: enough items to fill the chip several times over, each long enough to pay for staging its queries
     long long work = 0;
     for (long long g = 0; g < ngroups; ++g)
@@ -996,7 +1110,7 @@ int rag_mx4_scores_grouped_device(const rag_mx4_store_t* st, int64_t nq, const v
     if (widest < 1 || widest > nq) return fail(RAG_ERR_INVALID, "widest is not what rag_mx4_plan_groups gave for these queries");
     Mx4DeviceGuard g(st->device);
     if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
-    const Mx4Shape p = mx4_shape(q_type, st->dim, widest);
+    const Mx4Shape p = mx4_shape(q_type, st->dim, widest, total > MX4_WIDE);
     Mx4ScoreArgs a = mx4_score_args(st, p, q_dev, q_type, q_stride, normalize ? 1 : 0, out_dev);
     a.items = static_cast<const Mx4Item*>(items_dev);
     a.nq = (int)nq;

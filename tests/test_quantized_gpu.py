@@ -262,6 +262,48 @@ def test_cosine_scores(dtype):
     assert np.array_equal(zero, np.zeros((2, 600), np.float32))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nq,n,dim", [(1, 1_100_003, 100), (3, 1_050_017, 128), (4, 530_001, 200), (8, 360_031, 384), (5, 180_050, 700),
+                                      (16, 360_033, 350), (30, 180_063, 768), (2, 150_035, 1000), (9, 150_001, 1024), (1, 70_033, 2048),
+                                      (7, 60_011, 2500), (20, 140_007, 1024), (3, 36_003, 4200)])
+def test_scores_of_stores_beyond_the_caches(nq, n, dim, dtype):
+    """Stores over 64 MiB take kernels of their own; their scores are those of any part of the store, which a smaller one holds."""
+    rng = np.random.default_rng(nq + n + dim)
+    small, v = _index(rng, 4099, dim)
+    import torch
+    from rag_amd import QuantizedIndex
+    codes, scales = small.packed()
+    at = torch.from_numpy(rng.integers(0, 4099, n)).cuda()
+    index = QuantizedIndex.from_packed(codes[at], scales[at], dim)
+    assert index._codes.numel() > 64 << 20
+    q, q64 = _rows(rng, nq, dim, dtype)
+    part = small.scores(q)
+    _check_scores(part.cpu().numpy(), q64, v, dtype)
+    assert torch.equal(index.scores(q), part[:, at])
+    b = 1017                                                 # a range that begins inside a block of sixteen rows and ends inside one
+    assert torch.equal(index.scores(q, b, n - 3), part[:, at[b:n - 3]])
+
+
+def test_a_result_whose_rows_lie_far_apart():
+    """Scores of several queries more than 2^31 bytes apart: through the C entry point with a long out_stride."""
+    import ctypes as C
+    import torch
+    from rag_amd import _lib
+    rng = np.random.default_rng(31)
+    for dim, nq in ((96, 9), (300, 20)):
+        index, _ = _index(rng, 3000, dim)
+        for dtype in TYPES:
+            q, _ = _rows(rng, nq, dim, dtype)
+            want = index.scores(q)
+            stride = 700_000_000
+            out = torch.empty((nq - 1) * stride + 3000, dtype=torch.float32, device="cuda")
+            _lib.check(_lib.lib.rag_mx4_scores_device(C.byref(index._st), 0, 3000, nq, q.data_ptr(), TYPES.index(dtype), dim, 0, out.data_ptr(),
+                                                      stride, torch.cuda.current_stream().cuda_stream))
+            for i in range(nq):
+                assert torch.equal(out[i * stride: i * stride + 3000], want[i]), (dtype, i)
+            del out
+
+
 def test_queries_that_lie_apart_and_host_queries():
     import torch
     rng = np.random.default_rng(2)
