@@ -481,7 +481,8 @@ int rag_mx4_scores_device(const rag_mx4_store_t* st, int64_t row_begin, int64_t 
  * groups[4g + 3]) (groups may share queries and rows, and be empty); its scores, [queries][rows], follow those of group g - 1 in out_dev.  rag_mx4_plan_groups
  * (host memory, no GPU) checks the groups and cuts them into pieces of RAG_MX4_ITEM_BYTES for the kernel:
  *   items_out   max_items pieces; *n_items says how many there are (more than max_items: call again with room for them)
- *   out_begin   NULL or, per group, where its scores start;  *total: how many there are;  *widest: for the product call
+ *   out_begin   NULL or, per group, where its scores start;  *total: how many there are;  *widest: most queries of
+ *               a piece, for the product call
  * The pieces, copied to device memory, serve any number of products with queries of this count and type over a store
  * of at least n rows; a piece that does not fit the store, the queries or the `total` scores of out_dev is left out. */
 #define RAG_MX4_ITEM_BYTES 32

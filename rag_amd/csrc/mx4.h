@@ -34,4 +34,30 @@ struct Mx4Item {
 };
 static_assert(sizeof(Mx4Item) == 32, "RAG_MX4_ITEM_BYTES");
 
+struct Mx4ScoreArgs {
+    const uint8_t* codes;        // of the store's first row
+    const uint8_t* scales;
+    const void* q;
+    long long ldq;               // elements
+    int q_type, q_vec, dim, ks, ksu, code_ld, scale_ld, normalize;
+    unsigned per;                        // ceil(2^32 / (32 ks)): the query of a unit of 4 elements by a multiplication
+    size_t code_bytes, scale_bytes;      // of the whole store
+    float* out;
+    // grouped: one workgroup per item
+    const Mx4Item* items;
+    // dense: rows [row0, row0 + rows) cut into slabs, every slab against blocks of QB queries
+    long long row0, rows, slab, slabs, out_ld;
+    long long total;             // grouped: scores in out (and rows = the store's)
+    int nq, nqb;
+};
+
+// Which kernel a product takes: from the queries that meet a row, and the row's length.
+struct Mx4Shape {
+    int nd, mt, nb, u, nw, steps, ksu, qb;
+    bool big;
+    size_t lds;
+};
+int mx4_launch_f32(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s);      // mx4_scores_f32.hip
+int mx4_launch_16(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s);       // mx4_scores_16.hip
+
 }  // namespace rag

@@ -1,0 +1,97 @@
+// What the kernels over four-bit rows share: vector types, elements of the three float types, small reductions.
+#pragma once
+#include <type_traits>
+
+#include "index.h"
+#include "mx4.h"
+
+namespace rag {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F f) {
+    if constexpr (N > 0) {
+        static_for<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+
+__device__ __forceinline__ float mx4_pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // -126 <= e <= 127
+__device__ __forceinline__ float bf16_f32(unsigned h) { return __uint_as_float(h << 16); }
+__device__ __forceinline__ float f16_f32(unsigned short h) {
+    _Float16 v;
+    __builtin_memcpy(&v, &h, 2);
+    return (float)v;
+}
+// element i of a row of the given type (RAG_MX4_F32 / BF16 / F16)
+__device__ __forceinline__ float mx4_elem(const void* row, int type, long long i) {
+    if (type == RAG_MX4_F32) return static_cast<const float*>(row)[i];
+    const unsigned short h = static_cast<const unsigned short*>(row)[i];
+    return type == RAG_MX4_BF16 ? bf16_f32(h) : f16_f32(h);
+}
+// N (4 or 8) consecutive elements from i on; past `dim` zero.  vec: rows start on 16-byte boundaries.  ONCE: read past the
+// caches' retention, for rows that nobody reads again (writing 100k rows of 384 fp32: 43 -> 35 us).
+template <int N, bool ONCE = false>
+__device__ __forceinline__ void mx4_load(const void* row, int type, int i, int dim, int vec, float* v) {
+    if (vec && i + N <= dim) {
+        if (type == RAG_MX4_F32) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(row) + i + j);
+                const v4f x = ONCE ? __builtin_nontemporal_load(p) : *p;
+                v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
+            }
+        } else {
+            unsigned w[N / 2];
+            if constexpr (N == 8) {
+                const v4i* p = reinterpret_cast<const v4i*>(static_cast<const unsigned short*>(row) + i);
+                const v4i x = ONCE ? __builtin_nontemporal_load(p) : *p;
+                w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+            } else {
+                const v2u x = *reinterpret_cast<const v2u*>(static_cast<const unsigned short*>(row) + i);
+                w[0] = x.x; w[1] = x.y;
+            }
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) {
+                v[2 * j] = type == RAG_MX4_BF16 ? bf16_f32(w[j] & 0xffffu) : f16_f32((unsigned short)w[j]);
+                v[2 * j + 1] = type == RAG_MX4_BF16 ? __uint_as_float(w[j] & 0xffff0000u) : f16_f32((unsigned short)(w[j] >> 16));
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = i + j < dim ? mx4_elem(row, type, i + j) : 0.f;
+}
+
+__device__ __forceinline__ unsigned dpp_max_u32(unsigned v, unsigned o) { return v > o ? v : o; }
+// the largest of |v| (as ordered bits) over each aligned group of 4 / 8 lanes
+__device__ __forceinline__ unsigned quad_max(unsigned v) {
+    v = dpp_max_u32(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+    return dpp_max_u32(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
+}
+__device__ __forceinline__ unsigned oct_max(unsigned v) {
+    v = quad_max(v);
+    return dpp_max_u32(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));   // row_half_mirror
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+// 1 / |x| of one row by one wave: the sum of squares in fp64, rounded once (a zero row keeps its zeros)
+__device__ __forceinline__ float wave_inv_norm(const void* row, int type, int dim, int lane) {
+    double ss = 0.0;
+    for (int i = lane; i < dim; i += 64) {
+        const double x = (double)mx4_elem(row, type, i);
+        ss = fma(x, x, ss);
+    }
+    ss = wave_sum_f64(ss);
+    return ss > 0.0 ? (float)(1.0 / sqrt(ss)) : ss == 0.0 ? 1.f : (float)ss;      // NaN stays NaN
+}
+
+}  // namespace rag

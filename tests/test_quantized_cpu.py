@@ -45,7 +45,7 @@ def test_pieces_cover_every_score_of_every_group_once(seed):
     assert rc == 0 and 0 <= count <= 100_000
     sizes = (groups[:, 1] - groups[:, 0]) * (groups[:, 3] - groups[:, 2])
     assert total == sizes.sum() and np.array_equal(begin, np.cumsum(sizes) - sizes)
-    assert widest == max([int(q) for q, r in zip(groups[:, 1] - groups[:, 0], groups[:, 3] - groups[:, 2]) if r > 0], default=0)
+    assert widest == max([int(n) for n in items[:count]["nq"]], default=0)
     want_q, want_r = np.full(total, -1), np.full(total, -1)
     for (q0, q1, r0, r1), o in zip(groups, begin):
         want_q[o:o + (q1 - q0) * (r1 - r0)] = np.repeat(np.arange(q0, q1), r1 - r0)

@@ -263,11 +263,11 @@ def test_cosine_scores(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("nq,n,dim", [(1, 1_100_003, 100), (3, 1_050_017, 128), (4, 530_001, 200), (8, 360_031, 384), (5, 180_050, 700),
-                                      (16, 360_033, 350), (30, 180_063, 768), (2, 150_035, 1000), (9, 150_001, 1024), (1, 70_033, 2048),
-                                      (7, 60_011, 2500), (20, 140_007, 1024), (3, 36_003, 4200)])
+@pytest.mark.parametrize("nq,n,dim", [(1, 3_500_003, 100), (3, 3_400_017, 128), (4, 1_900_001, 200), (8, 1_300_031, 384), (5, 800_050, 700),
+                                      (16, 1_300_033, 350), (30, 700_063, 768), (2, 600_035, 1000), (9, 500_001, 1024), (1, 300_033, 2048),
+                                      (7, 262_171, 2500), (20, 500_007, 1024), (3, 262_145, 4200)])
 def test_scores_of_stores_beyond_the_caches(nq, n, dim, dtype):
-    """Stores over 64 MiB take kernels of their own; their scores are those of any part of the store, which a smaller one holds."""
+    """Stores over 256 MiB take kernels of their own; their scores are those of any part of the store, which a smaller one holds."""
     rng = np.random.default_rng(nq + n + dim)
     small, v = _index(rng, 4099, dim)
     import torch
@@ -275,7 +275,7 @@ def test_scores_of_stores_beyond_the_caches(nq, n, dim, dtype):
     codes, scales = small.packed()
     at = torch.from_numpy(rng.integers(0, 4099, n)).cuda()
     index = QuantizedIndex.from_packed(codes[at], scales[at], dim)
-    assert index._codes.numel() > 64 << 20
+    assert n * (index._code_bytes + index._scale_bytes) > 256 << 20
     q, q64 = _rows(rng, nq, dim, dtype)
     part = small.scores(q)
     _check_scores(part.cpu().numpy(), q64, v, dtype)
