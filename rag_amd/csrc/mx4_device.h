@@ -1,5 +1,8 @@
 // What the kernels over four-bit rows share: vector types, elements of the three float types, small reductions.
 #pragma once
+#include <float.h>
+#include <math.h>
+
 #include <type_traits>
 
 #include "index.h"
@@ -91,7 +94,7 @@ __device__ __forceinline__ float wave_inv_norm(const void* row, int type, int di
         ss = fma(x, x, ss);
     }
     ss = wave_sum_f64(ss);
-    return ss > 0.0 ? (float)(1.0 / sqrt(ss)) : ss == 0.0 ? 1.f : (float)ss;      // NaN stays NaN
+    return ss > 0.0 ? (float)fmin(1.0 / sqrt(ss), (double)FLT_MAX) : ss == 0.0 ? 1.f : (float)ss;      // NaN stays NaN
 }
 
 }  // namespace rag

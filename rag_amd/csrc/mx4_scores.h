@@ -36,7 +36,8 @@ struct Mx4Digits {
 // queries [q0, q0 + nqh) -> digit fragments in LDS.  frag[(block * TILES + tile) * 2 + half][place of lane][16 bytes], then the scales
 // sc[(block / 4) * TILES + tile][lane][block % 4], then 1 / |q|.  Blocks past the row's are zero: they meet a real block of the
 // row again.  A lane's place: its row number exclusive-or'ed with column and half, so that the lanes that write one digit of
-// consecutive elements meet different banks (with the rows in order sixteen lanes shared four).  What the fragments of absent queries hold does not matter: it stays in result rows that nobody reads.
+// consecutive elements meet different banks (with the rows in order sixteen lanes shared four).  What the fragments of absent
+// queries hold does not matter: it stays in result rows that nobody reads.
 template <int ND, int MT, int NT>
 __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long long q0, int nqh, uint8_t* frag, uint8_t* sc, float* inv) {
     typedef Mx4Digits<ND, MT> L;

@@ -403,6 +403,46 @@ def test_grouped_scores(ngroups, most_q, most_r, dim, nq, dtype):
     _check_scores(full, q64, v, dtype)
 
 
+def test_groups_of_very_many_scores():
+    """More than 10^8 scores: pieces for the kernels that reach results any distance apart."""
+    import torch
+    from rag_amd import QuantizedIndex
+    rng = np.random.default_rng(41)
+    small, _ = _index(rng, 4096, 32)
+    codes, scales = small.packed()
+    n = 26_000_000
+    at = torch.from_numpy(rng.integers(0, 4096, n)).cuda()
+    index = QuantizedIndex.from_packed(codes[at], scales[at], 32)
+    for dtype in TYPES:
+        q, _ = _rows(rng, 11, 32, dtype)
+        groups = np.array([[0, 3, 5, n - 7], [2, 11, 17, 3000], [10, 11, 0, n]])
+        plan = index.plan_groups(groups, 11, q.dtype)
+        assert plan.total > 100_000_000
+        part = small.scores(q)
+        for got, (q0, q1, r0, r1) in zip(plan.split(index.scores_grouped(q, plan)), groups):
+            assert torch.equal(got, part[q0:q1][:, at[r0:r1]])
+
+
+def test_rows_and_queries_of_extreme_norms():
+    """COSINE: norms whose reciprocal, or whose square, fp32 does not hold."""
+    import torch
+    from rag_amd import QuantizedIndex
+    rng = np.random.default_rng(42)
+    x = rng.standard_normal((6, 64)).astype(np.float32)
+    scale = np.array([1e-44, 1e-38, 1e-30, 1.0, 1e30, 1e37], np.float32)[:, None]
+    index = QuantizedIndex(64)
+    index.add(torch.from_numpy(x * scale).cuda())
+    s = index.scores(torch.from_numpy(x * scale).cuda()).cpu().numpy()
+    assert np.isfinite(s).all()
+    D, I = index.search(torch.from_numpy(x[2:]).cuda(), 1)
+    assert I[:, 0].tolist() == [2, 3, 4, 5]
+    codes, scales = index.packed()
+    unit = x.astype(np.float64) / np.linalg.norm(x.astype(np.float64), axis=1, keepdims=True)
+    want = mx4.scores(unit, mx4.values(codes.cpu().numpy(), scales.cpu().numpy(), 64))
+    # as in _check_scores, with the queries' norms rounded once more by the fp32 scaling of the inputs here
+    assert (np.abs(s - want)[2:, 2:] <= (12 * 16 / 15 + 4) * 2.0 ** -24 * (np.abs(unit) @ np.abs(mx4.values(codes.cpu().numpy(), scales.cpu().numpy(), 64)).T)[2:, 2:]).all()
+
+
 def test_pieces_that_do_not_fit_are_left_out():
     """Through the C entry point: pieces for other sizes write nothing, the others their scores."""
     import ctypes as C
