@@ -483,11 +483,13 @@ int rag_mx4_scores_device(const rag_mx4_store_t* st, int64_t row_begin, int64_t 
  *   items_out   max_items pieces; *n_items says how many there are (more than max_items: call again with room for them)
  *   out_begin   NULL or, per group, where its scores start;  *total: how many there are;  *widest: most queries of
  *               a piece, for the product call
- * The pieces, copied to device memory, serve any number of products with queries of this count and type over a store
+ * rag_mx4_upload_groups copies the pieces to device memory, enqueued on `stream` (refused while that is captured into a graph);
+ * `items` may be changed once it returns.  There they serve any number of products with queries of this count and type over a store
  * of at least n rows; a piece that does not fit the store, the queries or the `total` scores of out_dev is left out. */
 #define RAG_MX4_ITEM_BYTES 32
 int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngroups, const int64_t* groups, int64_t max_items,
                         void* items_out, int64_t* n_items, int64_t* out_begin, int64_t* total, int32_t* widest);
+int rag_mx4_upload_groups(const void* items, int64_t n_items, void* items_dev, int device, void* stream);
 int rag_mx4_scores_grouped_device(const rag_mx4_store_t* st, int64_t nq, const void* q_dev, int q_type, int64_t q_stride, int normalize,
                                   const void* items_dev, int64_t n_items, int32_t widest, float* out_dev, int64_t total, void* stream);
 /* rag_index_search_device over such a store: the k best of every query under the scores above, with the library's order rule

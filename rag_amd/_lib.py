@@ -90,6 +90,7 @@ SIGNATURES = {
     "rag_mx4_scores_device": (_i32, [_vp, _i64, _i64, _i64, _vp, _i32, _i64, _i32, _vp, _i64, _vp]),
     "rag_mx4_plan_groups": (_i32, [_i32, _i32, _i64, _i64, _i64, _vp, _i64, _vp, C.POINTER(_i64), _vp, C.POINTER(_i64),
                                    C.POINTER(_i32)]),
+    "rag_mx4_upload_groups": (_i32, [_vp, _i64, _vp, _i32, _vp]),
     "rag_mx4_scores_grouped_device": (_i32, [_vp, _i64, _vp, _i32, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _vp]),
     "rag_mx4_search_workspace": (_i64, [_i64, _i64, _i32]),
     "rag_mx4_search_device": (_i32, [_vp, _i64, _vp, _i32, _i64, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),

@@ -71,16 +71,18 @@ class GroupPlan:
         count, total, widest = C.c_int64(0), C.c_int64(0), C.c_int32(0)
         room = 2 * g.shape[0] + 64
         while True:
-            staging = torch.empty((room, _lib.MX4_ITEM_BYTES), dtype=torch.uint8, pin_memory=True)
-            check(lib.rag_mx4_plan_groups(self.dim, self.type, self.nq, self.n, g.shape[0], g.ctypes.data, room, staging.data_ptr(),
+            staging = np.empty((room, _lib.MX4_ITEM_BYTES), dtype=np.uint8)
+            check(lib.rag_mx4_plan_groups(self.dim, self.type, self.nq, self.n, g.shape[0], g.ctypes.data, room, staging.ctypes.data,
                                           C.byref(count), self.out_begin.ctypes.data, C.byref(total), C.byref(widest)))
             if count.value <= room:
                 break
             room = count.value
         self.total, self.widest, self.n_items = total.value, widest.value, count.value
         self._kept = _Kept(self.device)
-        self.items = staging[:self.n_items].to(torch.device("cuda", self.device), non_blocking=True)
+        self.items = torch.empty((self.n_items, _lib.MX4_ITEM_BYTES), dtype=torch.uint8, device=torch.device("cuda", self.device))
         self._kept.tensors = [self.items]
+        if self.n_items:
+            check(lib.rag_mx4_upload_groups(staging.ctypes.data, self.n_items, self.items.data_ptr(), self.device, self._kept.made_on))
 
     @property
     def shapes(self):

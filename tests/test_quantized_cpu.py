@@ -109,7 +109,10 @@ def test_arguments_are_refused_before_a_device_is_touched():
     for args in ((1, p, 0, 384, 0, 0, 0.0, None, None, p, p), (1, p, 0, 384, 0, 1025, 0.0, None, None, p, p),
                  (1, p, 0, 384, 0, 10, float("nan"), None, None, p, p), (1, p, 0, 384, 0, 10, 0.0, None, None, None, p)):
         assert lib.rag_mx4_search_device(ref, *args, p, 1 << 40, None) == bad, args
+    for args in ((p, -1, p), (p, 1, None), (None, 1, p), (p, 1, p + 8)):
+        assert lib.rag_mx4_upload_groups(*args, 0, None) == bad, args
     # nothing to do is no error
+    assert lib.rag_mx4_upload_groups(None, 0, None, 0, None) == 0
     assert lib.rag_mx4_scores_device(ref, 5, 5, 1, p, 0, 384, 0, None, 0, None) == 0
     assert lib.rag_mx4_scores_device(ref, 0, 100, 0, None, 0, 0, 0, None, 100, None) == 0
     assert lib.rag_mx4_write_device(ref, 100, None, None, 0, None, 0, 384, 0, None) == 0

@@ -468,6 +468,31 @@ def test_pieces_that_do_not_fit_are_left_out():
     assert np.array_equal(got, expect)
 
 
+def test_many_plans_on_their_way_at_once():
+    """More plans than there are blocks to copy them through, behind work that keeps the stream busy, and one too long for a block."""
+    import torch
+    rng = np.random.default_rng(23)
+    index, _ = _index(rng, 9000, 64)
+    q, _ = _rows(rng, 6, 64)
+    full = index.scores(q)
+    busy = torch.randn((4096, 4096), device="cuda")
+    for _ in range(40):
+        busy = busy @ busy * 1e-2
+    results = []
+    for i in range(150):
+        a = rng.integers(0, 9000, 8)
+        groups = np.stack([np.zeros(8, np.int64), rng.integers(1, 7, 8), a, np.minimum(9000, a + rng.integers(0, 400, 8))], 1)
+        results.append((groups, index.scores_grouped(q, groups)))
+    rows = np.arange(9000)
+    long = np.stack([rows % 6, rows % 6 + 1, rows, rows + 1], 1)
+    got = index.scores_grouped(q, long)
+    for groups, r in results:
+        want = torch.cat([full[b:e, c:d].reshape(-1) for b, e, c, d in groups.tolist()])
+        assert torch.equal(r, want)
+    at = torch.from_numpy(rows).cuda()
+    assert torch.equal(got, full[at % 6, at])
+
+
 def test_groups_are_planned_outside_of_a_capture():
     import torch
     rng = np.random.default_rng(22)
