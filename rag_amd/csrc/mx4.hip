@@ -49,10 +49,12 @@ struct Mx4WriteArgs {
     int upr;                     // units of 8 elements per (padded) row
     unsigned per;                // ceil(2^32 / upr): u / upr == (u * per) >> 32 for the units of a workgroup
     int per_block;               // rows a workgroup takes
+    long long block0;            // of the launch's first workgroup
 };
 constexpr int MX4_ROWS = 64;                 // most rows of one workgroup
 constexpr int MX4_FEW = 256;                 // up to so many positions a workgroup looks for repeated ones itself
 constexpr int MX4_UNITS = 4;
+constexpr long long MX4_GRID = 1 << 20;      // most workgroups of one launch: a launch has fewer than 2^32 threads
 
 // A position that is named twice keeps the last of its rows: the highest index wins the claim, whatever the order of arrival.
 __global__ __launch_bounds__(256) void mx4_claim_kernel(const long long* rows, long long count, long long n, int* owner) {
@@ -68,7 +70,7 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
     __shared__ long long s_to[MX4_ROWS];
     __shared__ float s_inv[MX4_ROWS];
     __shared__ int s_late[MX4_ROWS];
-    const long long i0 = (long long)blockIdx.x * a.per_block;
+    const long long i0 = (a.block0 + blockIdx.x) * a.per_block;
     const int nr = (int)(a.count - i0 < a.per_block ? a.count - i0 : a.per_block);
     const int tid = threadIdx.x, lane = tid & 63;
     constexpr size_t ESIZE = TYPE == RAG_MX4_F32 ? 4 : 2;
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
         for (int j = 0; j < MX4_UNITS; ++j) {
             const int u = u0 + 256 * j < units ? u0 + 256 * j : u0;
             const int r = (int)__umulhi((unsigned)u, a.per), c = u - r * a.upr;
-            if (!AT || s_to[r] >= 0) mx4_load<8, true>(x + (size_t)r * a.ldx * ESIZE, TYPE, c * 8, a.dim, VEC, v[j]);
+            if (!AT || s_to[r] >= 0) mx4_load8<TYPE, VEC>(x + (size_t)r * a.ldx * ESIZE, c * 8, a.dim, v[j]);
         }
 #pragma unroll
         for (int j = 0; j < MX4_UNITS; ++j) {
@@ -158,6 +160,7 @@ struct Mx4ReadArgs {
     int upr;
     unsigned per;                // as for writing; not used where upr is 1
     int per_block;
+    long long block0;
 };
 
 __device__ __forceinline__ unsigned pack16(int type, float lo, float hi) {
@@ -177,7 +180,7 @@ __device__ __forceinline__ unsigned pack16(int type, float lo, float hi) {
 template <int TYPE, bool VEC>
 __global__ __launch_bounds__(256) void mx4_read_kernel(Mx4ReadArgs a) {
     __shared__ long long s_from[MX4_ROWS];
-    const long long i0 = (long long)blockIdx.x * a.per_block;
+    const long long i0 = (a.block0 + blockIdx.x) * a.per_block;
     const int nr = (int)(a.count - i0 < a.per_block ? a.count - i0 : a.per_block);
     const int tid = threadIdx.x;
     if (tid < nr) {
@@ -279,16 +282,17 @@ static Mx4Shape mx4_shape_for(int type, int dim, long long nq, bool wide, Units 
 constexpr long long MX4_WIDE = 100 * 1000 * 1000;        // 3 * 4 bytes * this, and a tile, stay below 2^31
 
 static int mx4_launch_any(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s) {
-    if (grid < 1 || grid > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "four-bit product: grid out of range");
+    if (grid < 1 || grid * p.nw * 64 > 0xffffffffLL) return fail(RAG_ERR_INVALID, "four-bit product: grid out of range");
     return p.nd == 5 ? mx4_launch_f32(p, a, grid, device, s) : mx4_launch_16(p, a, grid, device, s);
 }
 
+static bool mx4_lies_on(const void* p, size_t boundary) { return (reinterpret_cast<uintptr_t>(p) & (boundary - 1)) == 0; }
 static int mx4_check_store(const rag_mx4_store_t* st) {
     if (!st) return fail(RAG_ERR_INVALID, "store is NULL");
     if (st->dim < 1 || st->dim > MX4_MAX_DIM) return fail(RAG_ERR_INVALID, "dim must be in [1, " + std::to_string(MX4_MAX_DIM) + "]");
     if (st->n < 0 || st->n > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "a store holds 0 to 2^31 - 1 rows");
     if (st->n > 0 && (!st->codes || !st->scales)) return fail(RAG_ERR_INVALID, "store without buffers");
-    if ((reinterpret_cast<uintptr_t>(st->codes) & 15) || (reinterpret_cast<uintptr_t>(st->scales) & 15))
+    if (!mx4_lies_on(st->codes, 16) || !mx4_lies_on(st->scales, 16))
         return fail(RAG_ERR_INVALID, "the store's buffers must lie on 16-byte boundaries");
     return RAG_OK;
 }
@@ -298,7 +302,7 @@ static int mx4_check_type(int type) {
 }
 static size_t mx4_esize(int type) { return type == RAG_MX4_F32 ? 4 : 2; }
 static int mx4_aligned(const void* p, long long ld, int type) {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (size_t)ld * mx4_esize(type) % 16 == 0;
+    return mx4_lies_on(p, 16) && (size_t)ld * mx4_esize(type) % 16 == 0;
 }
 // rows of a workgroup that writes or reads rows: four units a thread, fewer where that would leave compute units without work
 static int mx4_rows_per_block(long long count, int upr) {
@@ -436,7 +440,7 @@ static Mx4Slot* mx4_slot() {
         Mx4Slot& s = g_mx4_slots[(g_mx4_slot_next + i) % MX4_SLOTS];
         if (!s.host) {
             void* p = nullptr;
-            if (hipHostMalloc(&p, MX4_SLOT_BYTES + 64, hipHostMallocPortable) != hipSuccess) {
+            if (hipHostMalloc(&p, MX4_SLOT_BYTES + 64, hipHostMallocPortable | hipHostMallocCoherent) != hipSuccess) {
                 (void)hipGetLastError();
                 return nullptr;
             }
@@ -474,9 +478,10 @@ int rag_mx4_write_device(const rag_mx4_store_t* st, int64_t first, const int64_t
     if (count == 0) return RAG_OK;
     if (!x_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
     if (x_stride < st->dim) return fail(RAG_ERR_INVALID, "x_stride smaller than dim");
-    if ((reinterpret_cast<uintptr_t>(x_dev) & (mx4_esize(x_type) - 1))) return fail(RAG_ERR_INVALID, "x is not aligned to its elements");
+    if (!mx4_lies_on(x_dev, mx4_esize(x_type))) return fail(RAG_ERR_INVALID, "x is not aligned to its elements");
     if (rows_dev) {
         if (!owner_dev) return fail(RAG_ERR_INVALID, "positions need the store's owner array");
+        if (!mx4_lies_on(rows_dev, 8) || !mx4_lies_on(owner_dev, 4)) return fail(RAG_ERR_INVALID, "rows or owner is not aligned to its elements");
         if (st->n == 0) return RAG_OK;                  // every position lies outside
     } else if (first < 0 || first > st->n || count > st->n - first) {
         return fail(RAG_ERR_INVALID, "rows [first, first + count) do not lie inside the store");
@@ -505,18 +510,21 @@ int rag_mx4_write_device(const rag_mx4_store_t* st, int64_t first, const int64_t
         RAG_HIP_CHECK(hipGetLastError());
         a.owner = owner_dev;
     }
-    const dim3 grid((unsigned)((count + a.per_block - 1) / a.per_block));
+    const long long blocks = (count + a.per_block - 1) / a.per_block;
     const int vec = mx4_aligned(x_dev, x_stride, x_type);
+    for (; a.block0 < blocks; a.block0 += MX4_GRID) {
+        const dim3 grid((unsigned)std::min(MX4_GRID, blocks - a.block0));
 #define MX4_WRITE(T) \
-    if (x_type == T) { \
-        if (rows_dev && vec) hipLaunchKernelGGL((mx4_write_kernel<T, true, true>), grid, dim3(256), 0, s, a); \
-        else if (rows_dev) hipLaunchKernelGGL((mx4_write_kernel<T, false, true>), grid, dim3(256), 0, s, a); \
-        else if (vec) hipLaunchKernelGGL((mx4_write_kernel<T, true, false>), grid, dim3(256), 0, s, a); \
-        else hipLaunchKernelGGL((mx4_write_kernel<T, false, false>), grid, dim3(256), 0, s, a); \
-    }
-    MX4_WRITE(RAG_MX4_F32) MX4_WRITE(RAG_MX4_BF16) MX4_WRITE(RAG_MX4_F16)
+        if (x_type == T) { \
+            if (rows_dev && vec) hipLaunchKernelGGL((mx4_write_kernel<T, true, true>), grid, dim3(256), 0, s, a); \
+            else if (rows_dev) hipLaunchKernelGGL((mx4_write_kernel<T, false, true>), grid, dim3(256), 0, s, a); \
+            else if (vec) hipLaunchKernelGGL((mx4_write_kernel<T, true, false>), grid, dim3(256), 0, s, a); \
+            else hipLaunchKernelGGL((mx4_write_kernel<T, false, false>), grid, dim3(256), 0, s, a); \
+        }
+        MX4_WRITE(RAG_MX4_F32) MX4_WRITE(RAG_MX4_BF16) MX4_WRITE(RAG_MX4_F16)
 #undef MX4_WRITE
-    RAG_HIP_CHECK(hipGetLastError());
+        RAG_HIP_CHECK(hipGetLastError());
+    }
     return RAG_OK;
 }
 
@@ -526,7 +534,8 @@ int rag_mx4_read_device(const rag_mx4_store_t* st, const int64_t* rows_dev, int6
     if (count < 0 || count >= 0x7fffffffLL) return fail(RAG_ERR_INVALID, "count out of range");
     if (count == 0) return RAG_OK;
     if (!rows_dev || !out_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
-    if ((reinterpret_cast<uintptr_t>(out_dev) & (mx4_esize(out_type) - 1))) return fail(RAG_ERR_INVALID, "out is not aligned to its elements");
+    if (!mx4_lies_on(rows_dev, 8)) return fail(RAG_ERR_INVALID, "rows is not aligned to its elements");
+    if (!mx4_lies_on(out_dev, mx4_esize(out_type))) return fail(RAG_ERR_INVALID, "out is not aligned to its elements");
     Mx4DeviceGuard g(st->device);
     if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
     Mx4ReadArgs a = {};
@@ -542,17 +551,20 @@ int rag_mx4_read_device(const rag_mx4_store_t* st, const int64_t* rows_dev, int6
     a.upr = (st->dim + 7) / 8;
     a.per = (unsigned)((0x100000000ull + a.upr - 1) / a.upr);
     a.per_block = mx4_rows_per_block(count, a.upr);
-    const dim3 grid((unsigned)((count + a.per_block - 1) / a.per_block));
+    const long long blocks = (count + a.per_block - 1) / a.per_block;
     const int vec = st->dim % 8 == 0 && mx4_aligned(out_dev, st->dim, out_type);
     hipStream_t s = static_cast<hipStream_t>(stream);
+    for (; a.block0 < blocks; a.block0 += MX4_GRID) {
+        const dim3 grid((unsigned)std::min(MX4_GRID, blocks - a.block0));
 #define MX4_READ(T) \
-    if (out_type == T) { \
-        if (vec) hipLaunchKernelGGL((mx4_read_kernel<T, true>), grid, dim3(256), 0, s, a); \
-        else hipLaunchKernelGGL((mx4_read_kernel<T, false>), grid, dim3(256), 0, s, a); \
-    }
-    MX4_READ(RAG_MX4_F32) MX4_READ(RAG_MX4_BF16) MX4_READ(RAG_MX4_F16)
+        if (out_type == T) { \
+            if (vec) hipLaunchKernelGGL((mx4_read_kernel<T, true>), grid, dim3(256), 0, s, a); \
+            else hipLaunchKernelGGL((mx4_read_kernel<T, false>), grid, dim3(256), 0, s, a); \
+        }
+        MX4_READ(RAG_MX4_F32) MX4_READ(RAG_MX4_BF16) MX4_READ(RAG_MX4_F16)
 #undef MX4_READ
-    RAG_HIP_CHECK(hipGetLastError());
+        RAG_HIP_CHECK(hipGetLastError());
+    }
     return RAG_OK;
 }
 
@@ -562,7 +574,7 @@ static int mx4_check_queries(const rag_mx4_store_t* st, int64_t nq, const void* 
     if (nq < 0 || nq > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "nq out of range");
     if (nq > 0 && !q_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
     if (nq > 0 && q_stride < st->dim) return fail(RAG_ERR_INVALID, "q_stride smaller than dim");
-    if ((reinterpret_cast<uintptr_t>(q_dev) & (mx4_esize(q_type) - 1))) return fail(RAG_ERR_INVALID, "q is not aligned to its elements");
+    if (!mx4_lies_on(q_dev, mx4_esize(q_type))) return fail(RAG_ERR_INVALID, "q is not aligned to its elements");
     return RAG_OK;
 }
 
@@ -574,9 +586,15 @@ int rag_mx4_scores_device(const rag_mx4_store_t* st, int64_t row_begin, int64_t 
     if (nq == 0 || rows == 0) return RAG_OK;
     if (!out_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
     if (out_stride < rows) return fail(RAG_ERR_INVALID, "out_stride smaller than the number of rows");
+    if (!mx4_lies_on(out_dev, 4)) return fail(RAG_ERR_INVALID, "out is not aligned to its elements");
     Mx4DeviceGuard g(st->device);
     if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
-    return mx4_scores(st, row_begin, rows, nq, q_dev, q_type, q_stride, normalize ? 1 : 0, out_dev, out_stride, static_cast<hipStream_t>(stream));
+    constexpr int64_t most = 1 << 22;                           // queries of one launch (see MX4_GRID)
+    for (int64_t i = 0; i < nq; i += most)
+        if (int rc = mx4_scores(st, row_begin, rows, std::min(most, nq - i), static_cast<const char*>(q_dev) + (size_t)i * q_stride * mx4_esize(q_type),
+                                q_type, q_stride, normalize ? 1 : 0, out_dev + (size_t)i * out_stride, out_stride, static_cast<hipStream_t>(stream)))
+            return rc;
+    return RAG_OK;
 }
 
 int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngroups, const int64_t* groups, int64_t max_items,
@@ -611,29 +629,27 @@ int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngro
         return items;
     };
     const Mx4Shape p = mx4_shape_for(q_type, dim, std::max<long long>(most_q, 1), sum > MX4_WIDE, cut);       // (no group has more rows than scores)
-    cut(p);
+    const long long pieces = cut(p);
+    if (pieces > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "too many pieces");
     *widest = (int32_t)std::min<long long>(most_q, p.qb);
-    long long m = 0;
-    Mx4Item* items = static_cast<Mx4Item*>(items_out);
+    *n_items = pieces;
+    if (pieces > max_items) return RAG_OK;
+    Mx4Item* item = static_cast<Mx4Item*>(items_out);
     long long at = 0;
     for (long long g = 0; g < ngroups; ++g) {
         const int64_t* d = groups + 4 * g;
         const long long gq = d[1] - d[0], gr = d[3] - d[2];
         for (long long r = 0; r < gr && gq > 0; r += part)
-            for (long long q = 0; q < gq; q += p.qb, ++m)
-                if (m < max_items) {
-                    Mx4Item it;
-                    it.row0 = d[2] + r;
-                    it.at = at + q * gr + r;
-                    it.rows = (int)std::min(part, gr - r);
-                    it.ld = (int)gr;
-                    it.q0 = (int)(d[0] + q);
-                    it.nq = (int)std::min<long long>(p.qb, gq - q);
-                    items[m] = it;
-                }
+            for (long long q = 0; q < gq; q += p.qb, ++item) {
+                item->row0 = d[2] + r;
+                item->at = at + q * gr + r;
+                item->rows = (int)std::min(part, gr - r);
+                item->ld = (int)gr;
+                item->q0 = (int)(d[0] + q);
+                item->nq = (int)std::min<long long>(p.qb, gq - q);
+            }
         at += gq * gr;
     }
-    *n_items = m;
     return RAG_OK;
 }
 
@@ -641,7 +657,7 @@ int rag_mx4_upload_groups(const void* items, int64_t n_items, void* items_dev, i
     if (n_items < 0 || n_items > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "n_items out of range");
     if (n_items == 0) return RAG_OK;
     if (!items || !items_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
-    if ((reinterpret_cast<uintptr_t>(items_dev) & 15)) return fail(RAG_ERR_INVALID, "items must lie on a 16-byte boundary");
+    if (!mx4_lies_on(items_dev, 16)) return fail(RAG_ERR_INVALID, "items must lie on a 16-byte boundary");
     Mx4DeviceGuard g(device);
     if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -672,17 +688,21 @@ int rag_mx4_scores_grouped_device(const rag_mx4_store_t* st, int64_t nq, const v
     if (n_items < 0 || n_items > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "n_items out of range");
     if (n_items == 0) return RAG_OK;
     if (nq == 0 || !items_dev || !out_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
-    if ((reinterpret_cast<uintptr_t>(items_dev) & 15)) return fail(RAG_ERR_INVALID, "items must lie on a 16-byte boundary");
+    if (!mx4_lies_on(items_dev, 16)) return fail(RAG_ERR_INVALID, "items must lie on a 16-byte boundary");
+    if (!mx4_lies_on(out_dev, 4)) return fail(RAG_ERR_INVALID, "out is not aligned to its elements");
     if (widest < 1 || widest > nq) return fail(RAG_ERR_INVALID, "widest is not what rag_mx4_plan_groups gave for these queries");
     Mx4DeviceGuard g(st->device);
     if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
     const Mx4Shape p = mx4_shape(q_type, st->dim, mx4_tiles_for(q_type == RAG_MX4_F32 ? 5 : 4, widest), total > MX4_WIDE);
     Mx4ScoreArgs a = mx4_score_args(st, p, q_dev, q_type, q_stride, normalize ? 1 : 0, out_dev);
-    a.items = static_cast<const Mx4Item*>(items_dev);
     a.nq = (int)nq;
     a.rows = st->n;
     a.total = total;
-    return mx4_launch_any(p, a, n_items, st->device, static_cast<hipStream_t>(stream));
+    for (int64_t i = 0; i < n_items; i += MX4_GRID) {
+        a.items = static_cast<const Mx4Item*>(items_dev) + i;
+        if (int rc = mx4_launch_any(p, a, std::min<int64_t>(MX4_GRID, n_items - i), st->device, static_cast<hipStream_t>(stream))) return rc;
+    }
+    return RAG_OK;
 }
 
 int64_t rag_mx4_search_workspace(int64_t n, int64_t nq, int k) {
@@ -698,6 +718,7 @@ int rag_mx4_search_device(const rag_mx4_store_t* st, int64_t nq, const void* q_d
     if (min_score != min_score) return fail(RAG_ERR_INVALID, "min_score is NaN");
     if (nq == 0) return RAG_OK;
     if (!D_dev || !I_dev) return fail(RAG_ERR_INVALID, "NULL buffer");
+    if (!mx4_lies_on(D_dev, 4) || !mx4_lies_on(I_dev, 8)) return fail(RAG_ERR_INVALID, "D or I is not aligned to its elements");
     Mx4DeviceGuard g(st->device);
     if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -708,7 +729,7 @@ int rag_mx4_search_device(const rag_mx4_store_t* st, int64_t nq, const void* q_d
         return RAG_OK;
     }
     const Mx4Plan p = mx4_plan(st->n, nq, k);
-    if (!workspace_dev || (reinterpret_cast<uintptr_t>(workspace_dev) & 255) || workspace_bytes < (int64_t)p.total())
+    if (!workspace_dev || !mx4_lies_on(workspace_dev, 256) || workspace_bytes < (int64_t)p.total())
         return fail(RAG_ERR_INVALID, "workspace: " + std::to_string(p.total()) + " bytes on a 256-byte boundary are needed");
     char* w = static_cast<char*>(workspace_dev);
     float* scores = reinterpret_cast<float*>(w);

@@ -37,38 +37,30 @@ __device__ __forceinline__ float mx4_elem(const void* row, int type, long long i
     const unsigned short h = static_cast<const unsigned short*>(row)[i];
     return type == RAG_MX4_BF16 ? bf16_f32(h) : f16_f32(h);
 }
-// N (4 or 8) consecutive elements from i on; past `dim` zero.  vec: rows start on 16-byte boundaries.  ONCE: read past the
-// caches' retention, for rows that nobody reads again (writing 100k rows of 384 fp32: 43 -> 35 us).
-template <int N, bool ONCE = false>
-__device__ __forceinline__ void mx4_load(const void* row, int type, int i, int dim, int vec, float* v) {
-    if (vec && i + N <= dim) {
-        if (type == RAG_MX4_F32) {
+// Eight consecutive elements from i on; past `dim` zero.  VEC: rows start on 16-byte boundaries.  Read past the caches' retention:
+// nobody reads these rows again (writing 100k rows of 384 fp32: 43 -> 35 us).
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void mx4_load8(const void* row, int i, int dim, float* v) {
+    if (VEC && i + 8 <= dim) {
+        if constexpr (TYPE == RAG_MX4_F32) {
 #pragma unroll
-            for (int j = 0; j < N; j += 4) {
-                const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(row) + i + j);
-                const v4f x = ONCE ? __builtin_nontemporal_load(p) : *p;
+            for (int j = 0; j < 8; j += 4) {
+                const v4f x = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(static_cast<const float*>(row) + i + j));
                 v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
             }
         } else {
-            unsigned w[N / 2];
-            if constexpr (N == 8) {
-                const v4i* p = reinterpret_cast<const v4i*>(static_cast<const unsigned short*>(row) + i);
-                const v4i x = ONCE ? __builtin_nontemporal_load(p) : *p;
-                w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-            } else {
-                const v2u x = *reinterpret_cast<const v2u*>(static_cast<const unsigned short*>(row) + i);
-                w[0] = x.x; w[1] = x.y;
-            }
+            const v4i x = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(static_cast<const unsigned short*>(row) + i));
 #pragma unroll
-            for (int j = 0; j < N / 2; ++j) {
-                v[2 * j] = type == RAG_MX4_BF16 ? bf16_f32(w[j] & 0xffffu) : f16_f32((unsigned short)w[j]);
-                v[2 * j + 1] = type == RAG_MX4_BF16 ? __uint_as_float(w[j] & 0xffff0000u) : f16_f32((unsigned short)(w[j] >> 16));
+            for (int j = 0; j < 4; ++j) {
+                const unsigned w = (unsigned)x[j];
+                v[2 * j] = TYPE == RAG_MX4_BF16 ? bf16_f32(w & 0xffffu) : f16_f32((unsigned short)w);
+                v[2 * j + 1] = TYPE == RAG_MX4_BF16 ? __uint_as_float(w & 0xffff0000u) : f16_f32((unsigned short)(w >> 16));
             }
         }
         return;
     }
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = i + j < dim ? mx4_elem(row, type, i + j) : 0.f;
+    for (int j = 0; j < 8; ++j) v[j] = i + j < dim ? mx4_elem(row, TYPE, i + j) : 0.f;
 }
 
 __device__ __forceinline__ unsigned dpp_max_u32(unsigned v, unsigned o) { return v > o ? v : o; }

@@ -332,7 +332,7 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 columns_transpose(held[mt]);
-                const int r = (tile - 3) * 16, left = (rows - r) * 4 < 256 && rows - r < 64 ? (rows - r) * 4 : 256;
+                const int r = (tile - 3) * 16, left = rows - r < 64 ? (rows - r) * 4 : 256;
 #pragma unroll
                 for (int s = 0; s < QPT; ++s)
                     put(held[mt][s], out + (mt * QPT + s) * ld + r, mt * QPT + s < nqh ? left : 0, lane * 4);

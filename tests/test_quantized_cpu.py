@@ -122,6 +122,27 @@ def test_arguments_are_refused_before_a_device_is_touched():
     assert lib.rag_mx4_search_workspace(100, 1, 10) > 0
 
 
+def test_unaligned_buffers_are_refused():
+    p = 1 << 20
+    ref = C.byref(_lib.Mx4Store(p, p, 100, 384, 0))
+    bad = _lib.RAG_ERR_INVALID
+    assert lib.rag_mx4_scores_device(ref, 0, 10, 1, p, 0, 384, 0, p + 2, 10, None) == bad
+    assert lib.rag_mx4_scores_grouped_device(ref, 1, p, 0, 384, 0, p, 1, 1, p + 2, 100, None) == bad
+    assert lib.rag_mx4_write_device(ref, 0, p + 4, p, 1, p, 0, 384, 0, None) == bad
+    assert lib.rag_mx4_write_device(ref, 0, p, p + 2, 1, p, 0, 384, 0, None) == bad
+    assert lib.rag_mx4_read_device(ref, p + 4, 1, p, 0, None) == bad
+    assert lib.rag_mx4_search_device(ref, 1, p, 0, 384, 0, 10, 0.0, None, None, p + 2, p, p, 1 << 40, None) == bad
+    assert lib.rag_mx4_search_device(ref, 1, p, 0, 384, 0, 10, 0.0, None, None, p, p + 4, p, 1 << 40, None) == bad
+
+
+def test_more_pieces_than_a_plan_can_hold():
+    rc, *_ = _plan([[0, 2 ** 30, 0, 2 ** 29]], 2 ** 30, 2 ** 29)
+    assert rc == _lib.RAG_ERR_INVALID and "pieces" in _lib.last_error()
+    # many pieces, no room: the number comes without a walk over them
+    rc, items, count, _, total, widest = _plan([[0, 2 ** 10, 0, 2 ** 29]], 2 ** 10, 2 ** 29, kind=1, room=4)
+    assert rc == 0 and count == 2 ** 7 * 2 ** 16 and total == 2 ** 39 and widest == 8 and not items["rows"].any()
+
+
 def test_the_oracle_rounds_to_the_nearest_value():
     from oracle import mx4
     rng = np.random.default_rng(1)
