@@ -748,3 +748,193 @@ def test_refusals():
     with pytest.raises(RagHipError):
         index.search(x, 1, min_score=float("nan"))
     assert len(index) == 4
+
+
+# ------------------------------------------------------------------------------------------------ many rows, threads, streams
+def test_more_rows_than_one_launch_takes():
+    """Rows and positions beyond the workgroups of one launch (2^20 of 64 rows)."""
+    import torch
+    from rag_amd import QuantizedIndex
+    n = 64 * 2 ** 20 + 77
+    index = QuantizedIndex(1, metric="ip")
+    grid = torch.tensor([0.0, 1.0, 1.5, 2.0, -3.0, 0.75, -1.0, 6.0], dtype=torch.float16, device="cuda")     # each is kept exactly in a group of its own
+    x = grid[torch.randint(0, 8, (n, 1), device="cuda")]
+    index.add(x)
+    rows = torch.arange(n, device="cuda")
+    assert torch.equal(index.reconstruct(rows, dtype=torch.float16), x)
+    turn = rows.flip(0)
+    index.write(turn, x)
+    assert torch.equal(index.reconstruct(rows, dtype=torch.float16), x.flip(0))
+
+
+def test_more_groups_and_queries_than_one_launch_takes():
+    import torch
+    rng = np.random.default_rng(51)
+    index, _ = _index(rng, 700, 1)
+    q, _ = _rows(rng, 5, 1)
+    full = index.scores(q)
+    many = 2 ** 20 + 9                                                  # a piece each
+    a, b = rng.integers(0, 5, many), rng.integers(0, 700, many)
+    got = index.scores_grouped(q, np.stack([a, a + 1, b, b + 1], 1))
+    assert torch.equal(got, full[torch.from_numpy(a).cuda(), torch.from_numpy(b).cuda()])
+    at = torch.randint(0, 5, (2 ** 22 + 5,), device="cuda")
+    assert torch.equal(index.scores(q[at], 7, 9), full[at][:, 7:9])
+
+
+def test_an_index_of_too_many_rows_is_refused():
+    import torch
+    from rag_amd import QuantizedIndex
+    index = QuantizedIndex(1, metric="ip")
+    x = torch.ones((3, 1), dtype=torch.bfloat16, device="cuda")
+    index.add(x)
+    with pytest.raises(ValueError):
+        index.add(x[:1].expand(2 ** 31 - 2, 1))
+    assert len(index) == 3 and index.reconstruct([0, 1, 2]).ravel().tolist() == [1.0, 1.0, 1.0]
+
+
+def test_what_grows_is_refused_inside_a_capture():
+    import torch
+    rng = np.random.default_rng(52)
+    index, _ = _index(rng, 64, 64)
+    q, _ = _rows(rng, 2, 64)
+    x, _ = _rows(rng, 30, 64)
+    said = []
+    graph = torch.cuda.CUDAGraph()
+    before = index.packed()
+    with torch.cuda.graph(graph):
+        out = index.scores(q)
+        for call in (lambda: index.add(x), lambda: index.reserve(500), lambda: index.set_active([3], False)):
+            try:
+                call()
+            except ValueError as e:
+                said.append(str(e))
+    assert len(said) == 3 and all("outside of a graph capture" in s for s in said)
+    assert len(index) == 64 and torch.equal(index.packed()[0], before[0]) and torch.equal(index.packed()[1], before[1])
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(out, index.scores(q))
+    index.set_active([3], False)                                        # room for one more, but hidden rows
+    index.reserve(128)
+    graph = torch.cuda.CUDAGraph()
+    refused = False
+    with torch.cuda.graph(graph):
+        out = index.scores(q)
+        try:
+            index.add(x)
+        except ValueError:
+            refused = True
+    assert refused and len(index) == 64
+
+
+def test_an_index_that_grows_on_another_stream():
+    """Buffers that are given up while another stream still copies them are not handed out again before it has."""
+    import torch
+    rng = np.random.default_rng(53)
+    index, _ = _index(rng, 60_000, 64)
+    more, _ = _rows(rng, 40_000, 64)
+    index.set_active(np.arange(0, 60_000, 3), False)
+    index.add(more[:1])
+    codes, scales = index.packed()
+    size = index._codes.numel(), index._scales.numel()
+    busy = torch.randn((4096, 4096), device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(60):
+            busy = busy @ busy * 1e-2
+        index.add(more)
+        index.add(more)
+    trash = [torch.full((s,), 255, dtype=torch.uint8, device="cuda") for s in size for _ in range(3)]
+    trash += [torch.zeros((60_001,), dtype=torch.uint8, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    got = index.packed()
+    assert torch.equal(got[0][:60_001], codes) and torch.equal(got[1][:60_001], scales)
+    assert torch.equal(got[0][60_001:100_001], got[0][100_001:]) and len(index) == 140_001
+    I = index.search(more[:2], 1000)[1]
+    assert not ((I < 60_000) & (I % 3 == 0)).any() and (I >= 0).all()
+    del trash
+
+
+def test_a_plan_that_is_used_on_another_stream():
+    import torch
+    rng = np.random.default_rng(54)
+    index, _ = _index(rng, 5000, 64)
+    q, _ = _rows(rng, 4, 64)
+    groups = [[0, 4, 0, 5000], [1, 3, 17, 900]]
+    want = index.scores_grouped(q, groups)
+    busy = torch.randn((4096, 4096), device="cuda")
+    torch.cuda.synchronize()
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(first):
+        for _ in range(40):
+            busy = busy @ busy * 1e-2
+        plan = index.plan_groups(groups, 4)
+    with torch.cuda.stream(second):
+        got = index.scores_grouped(q, plan)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    # made on a stream of its own, used on the default one
+    with torch.cuda.stream(first):
+        plan = index.plan_groups(groups, 4)
+    assert torch.equal(index.scores_grouped(q, plan), want)
+    plan = index.plan_groups(groups, 4)
+    with torch.cuda.stream(second):
+        got = index.scores_grouped(q, plan)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_threads_share_an_index():
+    """Searches while another thread adds rows: every answer is that of the rows of some moment."""
+    import threading
+    import torch
+    rng = np.random.default_rng(55)
+    index, _ = _index(rng, 2000, 64)
+    q, _ = _rows(rng, 3, 64)
+    more, _ = _rows(rng, 500, 64)
+    answers, wrong = [], []
+    torch.cuda.synchronize()
+
+    def ask():
+        try:
+            for _ in range(60):
+                answers.append((len(index),) + index.search(q, 10) + (len(index),))
+        except Exception as e:                              # told below
+            wrong.append(e)
+
+    def grow():
+        try:
+            for _ in range(60):
+                index.add(more)
+        except Exception as e:
+            wrong.append(e)
+    threads = [threading.Thread(target=f) for f in (ask, grow, ask)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and len(index) == 32_000 and len(answers) == 120
+    full = index.scores(q)
+    for least, D, I, most in answers:
+        possible = []
+        for n in range(least, most + 1, 500):
+            top = torch.sort(full[:, :n], dim=1, descending=True, stable=True)
+            possible.append(torch.equal(D, top.values[:, :10]) and torch.equal(I, top.indices[:, :10]))
+        assert any(possible)
+
+
+def test_a_snapshot_whose_soft_deletes_do_not_fit(tmp_path):
+    from rag_amd import QuantizedIndex
+    rng = np.random.default_rng(56)
+    index, _ = _index(rng, 40, 64)
+    index.set_active([1, 2], False)
+    path = str(tmp_path / "rows")
+    index.save(path)
+    QuantizedIndex.load(path)
+    with np.load(path) as f:
+        kept = dict(f)
+    for active in (kept["active"][:39], kept["active"].astype(np.int64), np.ones((40, 2), np.uint8)):
+        with open(path, "wb") as f:
+            np.savez(f, **dict(kept, active=active))
+        with pytest.raises(ValueError):
+            QuantizedIndex.load(path)
