@@ -22,6 +22,8 @@ __host__ __device__ __forceinline__ int mx4_scale_at(int group) { return (group 
 
 constexpr int MX4_MAX_DIM = 8192;          // the query fragments of one matrix tile (2 KiB per block of 128) fit the LDS
 
+constexpr int MX4_FRAG = 1536;             // a block of one tile of query digits: 64 lanes of 32 six-bit values
+
 // One piece of the grouped product: `nq` queries from q0 against `rows` rows from row0; score (i, r) goes to
 // out[at + i * ld + r].  Written by rag_mx4_plan_groups, read by the kernel.
 struct Mx4Item {
@@ -40,7 +42,7 @@ struct Mx4ScoreArgs {
     const void* q;
     long long ldq;               // elements
     int q_type, q_vec, dim, ks, ksu, code_ld, scale_ld, normalize;
-    unsigned per;                        // ceil(2^32 / (32 ks)): the query of a unit of 4 elements by a multiplication
+    unsigned per;                        // ceil(2^32 / (4 ks)): the query of a group of 32 elements by a multiplication
     size_t code_bytes, scale_bytes;      // of the whole store
     float* out;
     // grouped: one workgroup per item

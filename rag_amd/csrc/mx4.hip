@@ -243,7 +243,7 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(Mx4ReadArgs a) {
 static int mx4_tiles(int nd, int mt) { return nd == 5 && mt > 1 ? mt + (mt + 3) / 4 : mt; }        // Mx4Digits::TILES
 static size_t mx4_lds(int ks, int u, int tiles) {
     const int ksu = (ks + u - 1) / u * u;
-    return (size_t)ksu * tiles * 2048 + (size_t)(ksu + 3) / 4 * tiles * 256 + (size_t)tiles * 4 * sizeof(float);
+    return (size_t)ksu * tiles * MX4_FRAG + (size_t)(ksu + 3) / 4 * tiles * 256 + (size_t)tiles * 4 * sizeof(float);
 }
 // tiles that nq queries fill
 static int mx4_tiles_for(int nd, long long nq) { return nq <= (nd == 5 ? 3 : 4) ? 1 : nq <= 8 ? 2 : nq <= 16 ? 4 : 8; }
@@ -320,7 +320,7 @@ static Mx4ScoreArgs mx4_score_args(const rag_mx4_store_t* st, const Mx4Shape& p,
     a.q_vec = mx4_aligned(q, ldq, q_type);
     a.dim = st->dim;
     a.ks = mx4_blocks(st->dim);
-    a.per = (unsigned)((0x100000000ull + 32 * a.ks - 1) / (32 * a.ks));
+    a.per = (unsigned)((0x100000000ull + 4 * a.ks - 1) / (4 * a.ks));
     a.ksu = p.ksu;
     a.code_ld = mx4_code_bytes(st->dim);
     a.scale_ld = mx4_scale_bytes(st->dim);

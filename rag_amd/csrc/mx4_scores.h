@@ -2,11 +2,13 @@
 // mx4_scores_16.hip.
 //
 // Products run on the scaled matrix instruction, which reads four-bit values and their scales as they are stored: nothing
-// is unpacked.  Its other operand is eight bits wide (e4m3, scaled per 32 as well), so a query is split into digits first:
+// is unpacked.  Its other operand is six bits wide (e2m3, scaled per 32 as well), so a query is split into digits first:
 // with 2^E the power of two that brings the largest element of a group of 32 into [8, 16),
 //     x = 2^E * (d0 + d1 / 32 + d2 / 32^2 + ...),   dj a whole number in [-16, 16],
-// and a whole number up to 16 is exact in e4m3.  Each digit is a row of the matrix tile of its own, with the scale
-// 2^(E - 5j), so one instruction multiplies all digits; the digits' sums are added at the end.  fp32 queries take five
+// and a whole number up to 16 is exact in e2m3, as so many eighths (its code is the number itself, and 32 where it is
+// negative).  With eight-bit digits the instruction takes twice as long and their fragments a third more of the LDS (256
+// fp32 queries x 200k x 768: 154 us, 134 with six; x 2048: 613, 399).  Each digit is a row of the matrix tile of its own, with the scale
+// 2^(E + 3 - 5j), so one instruction multiplies all digits; the digits' sums are added at the end.  fp32 queries take five
 // digits (what is left is at most 2^-24 of the group's largest element), bf16 and fp16 four (at most 2^-19 of it: every
 // element down to 2^-12 (bf16) / 2^-9 (fp16) of the largest one is exact).  Products of such digits with four-bit values
 // are multiples of 1/2 up to 96, which the instruction adds without loss; it adds across groups and to the accumulator in
@@ -16,12 +18,11 @@
 
 namespace rag {
 
-// Layout of the instruction (checked on the card): lane l, column c = l / 16.  Four-bit operand: row l % 16, elements
-// 32 c .. 32 c + 31 of the block of 128.  Eight-bit operand: row l % 16, bytes 0..15 = elements 16 c .., bytes 16..31 =
-// elements 64 + 16 c ..; scale of lane l (either operand): elements 32 c .. 32 c + 31.  Result register r of lane l:
-// (eight-bit row 4 c + r, four-bit row l % 16).
+// Layout of the instruction (checked on the card): lane l, column c = l / 16.  Either operand: row l % 16, elements
+// 32 c .. 32 c + 31 of the block of 128, and their scale.  Result register r of lane l: (row 4 c + r of the digits, row
+// l % 16 of the store).
 //
-// Digit j < 4 of query s of a tile is eight-bit row 4 s + j: the four registers of column s, added without leaving the lane.
+// Digit j < 4 of query s of a tile is row 4 s + j of the digits: the four registers of column s, added without leaving the lane.
 // Fifth digits (fp32): up to three queries share their tile with them -- rows 12 + s: register s of column 3, fetched from
 // there by fifth_digits().  More queries put four to a tile and have the fifth digits of each four tiles in one more tile, query s
 // of tile t in row 4 s + t: register t of column s, where they are wanted.
@@ -30,13 +31,102 @@ struct Mx4Digits {
     static constexpr bool INSIDE = ND == 5 && MT == 1;           // fifth digits in the tile itself
     static constexpr int EX = ND == 5 && !INSIDE ? (MT + 3) / 4 : 0;
     static constexpr int TILES = MT + EX;
-    static constexpr int QPT = INSIDE ? 3 : 4;                   // queries per tile of 16 eight-bit rows
+    static constexpr int QPT = INSIDE ? 3 : 4;                   // queries per tile of 16 rows of digits
 };
 
-// queries [q0, q0 + nqh) -> digit fragments in LDS.  frag[(block * TILES + tile) * 2 + half][place of lane][16 bytes], then the scales
-// sc[(block / 4) * TILES + tile][lane][block % 4], then 1 / |q|.  Blocks past the row's are zero: they meet a real block of the
-// row again.  A lane's place: its row number exclusive-or'ed with column and half, so that the lanes that write one digit of
-// consecutive elements meet different banks (with the rows in order sixteen lanes shared four).  What the fragments of absent
+// Unit u of the queries at q, EL consecutive elements, into the fragments.  The conversions round to nearest even, so a digit is
+// what a conversion makes of the rest, and the next rest is what is left of it, exactly.
+template <int ND, int MT, int EL>
+__device__ __forceinline__ void mx4_stage_unit(const Mx4ScoreArgs& a, const char* q, int u, uint8_t* frag, uint8_t* sc) {
+    typedef Mx4Digits<ND, MT> L;
+    constexpr int QPT = L::QPT, TILES = L::TILES, ESIZE = ND == 5 ? 4 : 2, SHARE = 32 / EL;
+    typedef typename std::conditional<EL * ESIZE % 16 == 0, v4i, v2i>::type Raw;
+    constexpr int PIECES = EL * ESIZE / sizeof(Raw), DW = sizeof(Raw) / 4;
+    // s: the query; its group of 32 elements; the lane's part `in` of that
+    const int ug = u / SHARE, in = u % SHARE, s = (int)__umulhi((unsigned)ug, a.per), group = ug - s * a.ks * 4, at0 = group * 32 + in * EL;
+    const char* row = q + (size_t)s * a.ldq * ESIZE;
+    float v[EL];
+    if (a.q_vec && at0 + EL <= a.dim) {
+        Raw raw[PIECES];
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) raw[j] = reinterpret_cast<const Raw*>(row + (size_t)at0 * ESIZE)[j];
+#pragma unroll
+        for (int j = 0; j < EL; ++j) {
+            if constexpr (ND == 5) v[j] = __int_as_float(raw[j / DW][j % DW]);
+            else {
+                const unsigned w = (unsigned)raw[j / 2 / DW][j / 2 % DW], h = j & 1 ? w >> 16 : w & 0xffffu;
+                v[j] = a.q_type == RAG_MX4_BF16 ? bf16_f32(h) : f16_f32((unsigned short)h);
+            }
+        }
+    } else {                                                    // unaligned, or the end of a row: zeros behind it
+#pragma unroll
+        for (int j = 0; j < EL; ++j) v[j] = at0 + j < a.dim ? mx4_elem(row, a.q_type, at0 + j) : 0.f;
+    }
+    unsigned most = 0;
+#pragma unroll
+    for (int j = 0; j < EL; ++j) {
+        const unsigned m = __float_as_uint(v[j]) & 0x7fffffffu;
+        most = m > most ? m : most;
+    }
+    if constexpr (SHARE == 8) most = oct_max(most);
+    const bool bad = most >= 0x7f800000u;
+    int e = (int)(most >> 23) - 130;                            // the largest element / 2^e lies in [8, 16)
+    e = e < -100 ? -100 : e;                                    // (a group below 2^-97 has its digits cut instead)
+    e = bad ? 0 : e;
+    const float down = mx4_pow2(-e);
+    const int block = group >> 2, col = group & 3, turn = col | (block & 3) << 2;
+    const int tile = s / QPT, slot = s - tile * QPT;
+    uint8_t* to = frag + (size_t)block * TILES * MX4_FRAG;
+    uint8_t* ts = sc + (size_t)((block >> 2) * TILES) * 256 + col * 64 + (block & 3);
+#pragma unroll
+    for (int j = 0; j < EL; ++j) v[j] *= down;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        const int m = d < 4 ? 4 * slot + d : L::INSIDE ? 12 + slot : 4 * slot + (tile & 3);
+        const int at = d < 4 || L::INSIDE ? tile : MT + (tile >> 2);
+        const int place = col * 16 + (m ^ turn);
+        uint8_t* first = to + at * MX4_FRAG + place * 16;
+        uint8_t* last = to + at * MX4_FRAG + 1024 + place * 8;
+        if constexpr (EL == 32) {
+            const float unit = mx4_pow2(3 - 5 * d);              // six-bit values are eighths
+            v16f even, odd;                                     // of the pairs that the conversion interleaves
+#pragma unroll
+            for (int j = 0; j < 16; ++j) { even[j] = v[2 * j]; odd[j] = v[2 * j + 1]; }
+            const v6u p = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, unit);
+            *reinterpret_cast<v4i*>(first) = (v4i){(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
+            *reinterpret_cast<v2u*>(last) = (v2u){p[4], p[5]};
+            if (d + 1 < ND) {
+                const v32f w = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(p, unit);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] -= w[j];
+            }
+        } else {
+            // by way of e4m3, whose lowest values (multiples of 2^-9, up to 16 of them) are sign and magnitude too
+            const float unit = mx4_pow2(9 - 5 * d);
+            v2s b = {0, 0};
+            b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(b, v[0], v[1], unit, false);
+            b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(b, v[2], v[3], unit, true);
+            const unsigned x = __builtin_bit_cast(unsigned, b);
+            if (d + 1 < ND) {
+                const v2f lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x, unit, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x, unit, true);
+                v[0] -= lo.x; v[1] -= lo.y; v[2] -= hi.x; v[3] -= hi.y;
+            }
+            // four codes in 24 bits; four lanes make three dwords of them
+            const unsigned y = (x & 0x1f1f1f1fu) | ((x >> 2) & 0x20202020u);
+            const unsigned p = __builtin_amdgcn_udot4(y, 0x4001u, 0u, false) | __builtin_amdgcn_udot4(y, 0x40010000u, 0u, false) << 12;
+            const unsigned next = (unsigned)__builtin_amdgcn_update_dpp(0, (int)p, 0xF9, 0xF, 0xF, true);      // of the lane behind this one
+            const int k = in & 3, n = 3 * (in >> 2) + k;         // dword of the lane's six
+            if (k < 3) *reinterpret_cast<unsigned*>(n < 4 ? first + 4 * n : last + 4 * (n - 4)) = p >> 8 * k | next << (24 - 8 * k);
+        }
+        // NaN: every score of the query is NaN
+        if (in == 0) ts[at * 256 + m * 4] = bad && d == 0 ? 255 : (uint8_t)(130 + e - 5 * d);
+    }
+}
+
+// queries [q0, q0 + nqh) -> digit fragments in LDS, 1536 bytes per block and tile: the first sixteen bytes of every lane, then the
+// last eight of every lane.  Behind them the scales sc[(block / 4) * TILES + tile][lane][block % 4], then 1 / |q|.  Blocks past the
+// row's are zero: they meet a real block of the row again.  A lane's place: its row number exclusive-or'ed with column and
+// block, so that the lanes that write one digit of consecutive elements meet different banks.  What the fragments of absent
 // queries hold does not matter: it stays in result rows that nobody reads.
 template <int ND, int MT, int NT>
 __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long long q0, int nqh, uint8_t* frag, uint8_t* sc, float* inv) {
@@ -45,103 +135,26 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long lo
     const int tid = threadIdx.x;
     if (a.ksu > a.ks) {
         const v4i zero = {0, 0, 0, 0};
-        v4i* f = reinterpret_cast<v4i*>(frag + (size_t)a.ks * TILES * 2048);
-        for (int i = tid; i < (a.ksu - a.ks) * TILES * 128; i += NT) f[i] = zero;
+        v4i* f = reinterpret_cast<v4i*>(frag + (size_t)a.ks * TILES * MX4_FRAG);
+        for (int i = tid; i < (a.ksu - a.ks) * TILES * (MX4_FRAG / 16); i += NT) f[i] = zero;
         v4i* s = reinterpret_cast<v4i*>(sc + (size_t)(a.ks / 4) * TILES * 256);
         for (int i = tid; i < ((a.ksu + 3) / 4 - a.ks / 4) * TILES * 16; i += NT) s[i] = zero;
         __syncthreads();
     }
-    const size_t esize = a.q_type == RAG_MX4_F32 ? 4 : 2;
-    const char* q = static_cast<const char*>(a.q) + (size_t)q0 * a.ldq * esize;
+    constexpr int ESIZE = ND == 5 ? 4 : 2;
+    const char* q = static_cast<const char*>(a.q) + (size_t)q0 * a.ldq * ESIZE;
     for (int s = tid >> 6; s < MT * QPT; s += NT / 64) {
         float f = 1.f;
-        if (a.normalize && s < nqh) f = wave_inv_norm(q + (size_t)s * a.ldq * esize, a.q_type, a.dim, tid & 63);
+        if (a.normalize && s < nqh) f = wave_inv_norm(q + (size_t)s * a.ldq * ESIZE, a.q_type, a.dim, tid & 63);
         if ((tid & 63) == 0) inv[s] = f;
     }
-    // units of 4 elements, 32 a block; the loads of two of them are under way at once
-    const int upq = a.ks * 32, units = nqh * upq;
-    constexpr int AHEAD = 2;
-    for (int u0 = tid; u0 < units; u0 += AHEAD * NT) {
-        float part[AHEAD][4];
-        if (a.q_vec) {
-            typedef typename std::conditional<ND == 5, v4f, v2u>::type Raw;
-            Raw raw[AHEAD];
-            bool whole[AHEAD];
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                const int u = u0 + i * NT < units ? u0 + i * NT : u0;
-                const int s = (int)__umulhi((unsigned)u, a.per), c = u - s * upq;
-                whole[i] = c * 4 + 4 <= a.dim;
-                raw[i] = Raw{};
-                if (whole[i]) raw[i] = *reinterpret_cast<const Raw*>(q + ((size_t)s * a.ldq + c * 4) * esize);
-            }
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if constexpr (ND == 5) part[i][j] = raw[i][j];
-                    else {
-                        const unsigned h = j & 1 ? raw[i][j >> 1] >> 16 : raw[i][j >> 1] & 0xffffu;
-                        part[i][j] = a.q_type == RAG_MX4_BF16 ? bf16_f32(h) : f16_f32((unsigned short)h);
-                    }
-                }
-                if (!whole[i]) {                                // the end of a row: element by element, zeros behind it
-                    const int u = u0 + i * NT < units ? u0 + i * NT : u0;
-                    const int s = (int)__umulhi((unsigned)u, a.per), c = u - s * upq;
-                    for (int j = 0; j < 4; ++j) part[i][j] = c * 4 + j < a.dim ? mx4_elem(q + (size_t)s * a.ldq * esize, a.q_type, c * 4 + j) : 0.f;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                const int u = u0 + i * NT < units ? u0 + i * NT : u0;
-                const int s = (int)__umulhi((unsigned)u, a.per), c = u - s * upq;
-                for (int j = 0; j < 4; ++j) part[i][j] = c * 4 + j < a.dim ? mx4_elem(q + (size_t)s * a.ldq * esize, a.q_type, c * 4 + j) : 0.f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int u = u0 + i * NT;
-            if (u >= units) break;
-            const int s = (int)__umulhi((unsigned)u, a.per), c = u - s * upq;
-            float* const v = part[i];
-            unsigned most = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const unsigned m = __float_as_uint(v[j]) & 0x7fffffffu;
-                most = m > most ? m : most;
-            }
-            most = oct_max(most);                               // eight lanes hold a group of 32
-            const bool bad = most >= 0x7f800000u;
-            int e = (int)(most >> 23) - 130;                    // the largest element / 2^e lies in [8, 16)
-            e = e < -100 ? -100 : e;                            // (a group below 2^-97 has its digits cut instead)
-            e = bad ? 0 : e;
-            const float down = mx4_pow2(-e);
-            const int block = c >> 5, in = c & 31;              // 4 elements `in` of the block
-            const int col = (in >> 2) & 3, half = in >> 4;
-            const int tile = s / QPT, slot = s - tile * QPT;
-            uint8_t* to = frag + (size_t)(block * TILES * 2 + half) * 1024 + col * 256 + (in & 3) * 4;
-            const int turn = col | half << 2;
-            uint8_t* ts = sc + (size_t)((block >> 2) * TILES) * 256 + (in >> 3) * 64 + (block & 3);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] *= down;
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                float w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    w[j] = rintf(v[j]);
-                    v[j] = (v[j] - w[j]) * 32.f;                // both steps exact
-                }
-                int p = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], 0, false);
-                p = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], p, true);
-                if (bad) p = d == 0 ? 0x7f7f7f7f : 0;           // NaN: every score of the query is NaN
-                const int m = d < 4 ? 4 * slot + d : L::INSIDE ? 12 + slot : 4 * slot + (tile & 3);
-                const int at = d < 4 || L::INSIDE ? tile : MT + (tile >> 2);
-                *reinterpret_cast<int*>(to + at * 2048 + (m ^ turn) * 16) = p;
-                if ((in & 7) == 0) ts[at * 256 + m * 4] = (uint8_t)(127 + e - 5 * d);
-            }
-        }
+    // A group of 32 elements to a lane is the least work (32 fp32 queries x 10k x 768: 7.7 us, 11.0 with four elements to a lane);
+    // where there are so few that the lanes take only part of one each, it is the sum of their latencies that counts
+    const int groups = nqh * a.ks * 4;
+    if (MT <= 2 && groups * 8 <= NT) {
+        if (tid < groups * 8) mx4_stage_unit<ND, MT, 4>(a, q, tid, frag, sc);
+    } else {
+        for (int u = tid; u < groups; u += NT) mx4_stage_unit<ND, MT, 32>(a, q, u, frag, sc);
     }
     __syncthreads();
 }
@@ -192,7 +205,7 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     const int ks = STEPS ? STEPS * U : a.ks, ksu = STEPS ? STEPS * U : a.ksu;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     uint8_t* frag = smem;
-    uint8_t* sc = frag + (size_t)ksu * TILES * 2048;
+    uint8_t* sc = frag + (size_t)ksu * TILES * MX4_FRAG;
     float* inv = reinterpret_cast<float*>(sc + (size_t)((ksu + 3) / 4) * TILES * 256);
 
     // rows [row0, row0 + rows) against queries [q0, q0 + nqh); this wave takes the tiles of 16 NB rows first, first + stride, ...
@@ -272,17 +285,19 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         constexpr bool FIRST = decltype(first_of_row)::value;   // begins the sums at zero
         constexpr bool SHIFT = STEPS == 0 && U < 4;             // the fetch may begin inside a scale dword
         constexpr int K0 = [] { if constexpr (STEPS) return decltype(ks0c)::value; else return 0; }();
-        const uint8_t* f = frag + (size_t)ks0 * TILES * 2048;
-        int fl = (col * 16 + (n16 ^ col)) * 16, sl = lane * 4;  // places of the first half; the second half's differ in bit 2 of the row
+        const uint8_t* f = frag + (size_t)ks0 * TILES * MX4_FRAG;
+        int fl = (col * 16 + (n16 ^ col)) * 16, sl = lane * 4;  // place in a block whose number is a multiple of 4
         if constexpr (TILES > 1) asm volatile("" : "+v"(fl), "+v"(sl));      // more than one tile's fragments do not fit the registers: read from LDS each time
         // query fragments AHEAD tiles ahead: the LDS latency passes under the products of the tiles before
         constexpr int AHEAD = 2, RING = AHEAD + 1;
-        v4i lo[RING], hi[RING];
+        v4i lo[RING];
+        v2u hi[RING];
         int xs[RING];
         auto fetch = [&](auto ic) {
             constexpr int i = decltype(ic)::value, u = i / TILES, mt = i % TILES;
-            lo[i % RING] = *reinterpret_cast<const v4i*>(f + i * 2048 + fl);
-            hi[i % RING] = *reinterpret_cast<const v4i*>(f + i * 2048 + 1024 + (fl ^ 64));
+            const int place = fl ^ ((SHIFT ? ks0 + u : K0 + u) & 3) << 6;
+            lo[i % RING] = *reinterpret_cast<const v4i*>(f + i * MX4_FRAG + place);
+            hi[i % RING] = *reinterpret_cast<const v2u*>(f + i * MX4_FRAG + 1024 + (place >> 1));
             const int x = *reinterpret_cast<const int*>(sc + (size_t)(((ks0 + (SHIFT ? 0 : u)) >> 2) * TILES + mt) * 256 + sl);
             xs[i % RING] = SHIFT ? (int)((unsigned)x >> ((ks0 & 3) * 8)) : x;
         };
@@ -299,12 +314,13 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
             constexpr int kk = K0 + u;                          // (K0 is a multiple of 4, or shifted away, where STEPS is 0)
             if constexpr (i + AHEAD < U * TILES) fetch(std::integral_constant<int, i + AHEAD>{});
             if constexpr (TILES > 1) __builtin_amdgcn_sched_barrier(0);
-            const v8i x = __builtin_shufflevector(lo[i % RING], hi[i % RING], 0, 1, 2, 3, 4, 5, 6, 7);
+            const v4i l = lo[i % RING];
+            const v8i x = {l.x, l.y, l.z, l.w, (int)hi[i % RING].x, (int)hi[i % RING].y, 0, 0};        // (24 bytes: the rest is not read)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const v8i y = __builtin_shufflevector(b.w[nb][u], b.w[nb][u], 0, 1, 2, 3, -1, -1, -1, -1);
                 const v4f c = FIRST && u == 0 ? (v4f){0.f, 0.f, 0.f, 0.f} : acc[mt][nb];
-                acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 4, kk & 3, xs[i % RING], kk & 3,
+                acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 2, 4, kk & 3, xs[i % RING], kk & 3,
                                                                                ys[nb][(kk >> 2) - (K0 >> 2)]);
             }
         });
