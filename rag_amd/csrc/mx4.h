@@ -23,6 +23,7 @@ __host__ __device__ __forceinline__ int mx4_scale_at(int group) { return (group 
 constexpr int MX4_MAX_DIM = 8192;          // the query fragments of one matrix tile (2 KiB per block of 128) fit the LDS
 
 constexpr int MX4_FRAG = 1536;             // a block of one tile of query digits: 64 lanes of 32 six-bit values
+__host__ __device__ constexpr int mx4_frag_ld(int tiles) { return tiles * MX4_FRAG + 64; }     // from block to block
 
 // One piece of the grouped product: `nq` queries from q0 against `rows` rows from row0; score (i, r) goes to
 // out[at + i * ld + r].  Written by rag_mx4_plan_groups, read by the kernel.

@@ -243,7 +243,7 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(Mx4ReadArgs a) {
 static int mx4_tiles(int nd, int mt) { return nd == 5 && mt > 1 ? mt + (mt + 3) / 4 : mt; }        // Mx4Digits::TILES
 static size_t mx4_lds(int ks, int u, int tiles) {
     const int ksu = (ks + u - 1) / u * u;
-    return (size_t)ksu * tiles * MX4_FRAG + (size_t)(ksu + 3) / 4 * tiles * 256 + (size_t)tiles * 4 * sizeof(float);
+    return (size_t)ksu * mx4_frag_ld(tiles) + (size_t)(ksu + 3) / 4 * tiles * 256 + (size_t)tiles * 4 * sizeof(float);
 }
 // tiles that nq queries fill
 static int mx4_tiles_for(int nd, long long nq) { return nq <= (nd == 5 ? 3 : 4) ? 1 : nq <= 8 ? 2 : nq <= 16 ? 4 : 8; }

@@ -74,9 +74,9 @@ __device__ __forceinline__ void mx4_stage_unit(const Mx4ScoreArgs& a, const char
     e = e < -100 ? -100 : e;                                    // (a group below 2^-97 has its digits cut instead)
     e = bad ? 0 : e;
     const float down = mx4_pow2(-e);
-    const int block = group >> 2, col = group & 3, turn = col | (block & 3) << 2;
+    const int block = group >> 2, col = group & 3;
     const int tile = s / QPT, slot = s - tile * QPT;
-    uint8_t* to = frag + (size_t)block * TILES * MX4_FRAG;
+    uint8_t* to = frag + block * mx4_frag_ld(TILES);
     uint8_t* ts = sc + (size_t)((block >> 2) * TILES) * 256 + col * 64 + (block & 3);
 #pragma unroll
     for (int j = 0; j < EL; ++j) v[j] *= down;
@@ -84,7 +84,7 @@ __device__ __forceinline__ void mx4_stage_unit(const Mx4ScoreArgs& a, const char
     for (int d = 0; d < ND; ++d) {
         const int m = d < 4 ? 4 * slot + d : L::INSIDE ? 12 + slot : 4 * slot + (tile & 3);
         const int at = d < 4 || L::INSIDE ? tile : MT + (tile >> 2);
-        const int place = col * 16 + (m ^ turn);
+        const int place = col * 16 + (m ^ col);
         uint8_t* first = to + at * MX4_FRAG + place * 16;
         uint8_t* last = to + at * MX4_FRAG + 1024 + place * 8;
         if constexpr (EL == 32) {
@@ -125,9 +125,9 @@ __device__ __forceinline__ void mx4_stage_unit(const Mx4ScoreArgs& a, const char
 
 // queries [q0, q0 + nqh) -> digit fragments in LDS, 1536 bytes per block and tile: the first sixteen bytes of every lane, then the
 // last eight of every lane.  Behind them the scales sc[(block / 4) * TILES + tile][lane][block % 4], then 1 / |q|.  Blocks past the
-// row's are zero: they meet a real block of the row again.  A lane's place: its row number exclusive-or'ed with column and
-// block, so that the lanes that write one digit of consecutive elements meet different banks.  What the fragments of absent
-// queries hold does not matter: it stays in result rows that nobody reads.
+// row's are zero: they meet a real block of the row again.  A lane's place is its row number exclusive-or'ed with the column,
+// and blocks lie 64 bytes more than their size apart, so that the lanes that write one digit of consecutive elements meet different
+// banks.  What the fragments of absent queries hold does not matter: it stays in result rows that nobody reads.
 template <int ND, int MT, int NT>
 __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long long q0, int nqh, uint8_t* frag, uint8_t* sc, float* inv) {
     typedef Mx4Digits<ND, MT> L;
@@ -135,8 +135,8 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, long lo
     const int tid = threadIdx.x;
     if (a.ksu > a.ks) {
         const v4i zero = {0, 0, 0, 0};
-        v4i* f = reinterpret_cast<v4i*>(frag + (size_t)a.ks * TILES * MX4_FRAG);
-        for (int i = tid; i < (a.ksu - a.ks) * TILES * (MX4_FRAG / 16); i += NT) f[i] = zero;
+        v4i* f = reinterpret_cast<v4i*>(frag + a.ks * mx4_frag_ld(TILES));
+        for (int i = tid; i < (a.ksu - a.ks) * (mx4_frag_ld(TILES) / 16); i += NT) f[i] = zero;
         v4i* s = reinterpret_cast<v4i*>(sc + (size_t)(a.ks / 4) * TILES * 256);
         for (int i = tid; i < ((a.ksu + 3) / 4 - a.ks / 4) * TILES * 16; i += NT) s[i] = zero;
         __syncthreads();
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     const int ks = STEPS ? STEPS * U : a.ks, ksu = STEPS ? STEPS * U : a.ksu;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     uint8_t* frag = smem;
-    uint8_t* sc = frag + (size_t)ksu * TILES * MX4_FRAG;
+    uint8_t* sc = frag + ksu * mx4_frag_ld(TILES);
     float* inv = reinterpret_cast<float*>(sc + (size_t)((ksu + 3) / 4) * TILES * 256);
 
     // rows [row0, row0 + rows) against queries [q0, q0 + nqh); this wave takes the tiles of 16 NB rows first, first + stride, ...
@@ -285,21 +285,25 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         constexpr bool FIRST = decltype(first_of_row)::value;   // begins the sums at zero
         constexpr bool SHIFT = STEPS == 0 && U < 4;             // the fetch may begin inside a scale dword
         constexpr int K0 = [] { if constexpr (STEPS) return decltype(ks0c)::value; else return 0; }();
-        const uint8_t* f = frag + (size_t)ks0 * TILES * MX4_FRAG;
-        int fl = (col * 16 + (n16 ^ col)) * 16, sl = lane * 4;  // place in a block whose number is a multiple of 4
-        if constexpr (TILES > 1) asm volatile("" : "+v"(fl), "+v"(sl));      // more than one tile's fragments do not fit the registers: read from LDS each time
+        const uint8_t* f = frag + ks0 * mx4_frag_ld(TILES);
+        int fl = (col * 16 + (n16 ^ col)) * 16, fh = 1024 + fl / 2, sl = lane * 4;
+        if constexpr (TILES > 1) asm volatile("" : "+v"(fl), "+v"(fh), "+v"(sl));      // more than one tile's fragments do not fit the registers: read from LDS each time
         // query fragments AHEAD tiles ahead: the LDS latency passes under the products of the tiles before
         constexpr int AHEAD = 2, RING = AHEAD + 1;
         v4i lo[RING];
         v2u hi[RING];
-        int xs[RING];
+        // scales: a dword covers four blocks, and is kept over them where it is not replaced before its last use (256 fp32 queries x
+        // 200k x 1536: 297 us, 283 like this)
+        constexpr bool KEEP = TILES > AHEAD;
+        int xs[KEEP ? TILES : RING];
         auto fetch = [&](auto ic) {
             constexpr int i = decltype(ic)::value, u = i / TILES, mt = i % TILES;
-            const int place = fl ^ ((SHIFT ? ks0 + u : K0 + u) & 3) << 6;
-            lo[i % RING] = *reinterpret_cast<const v4i*>(f + i * MX4_FRAG + place);
-            hi[i % RING] = *reinterpret_cast<const v2u*>(f + i * MX4_FRAG + 1024 + (place >> 1));
-            const int x = *reinterpret_cast<const int*>(sc + (size_t)(((ks0 + (SHIFT ? 0 : u)) >> 2) * TILES + mt) * 256 + sl);
-            xs[i % RING] = SHIFT ? (int)((unsigned)x >> ((ks0 & 3) * 8)) : x;
+            lo[i % RING] = *reinterpret_cast<const v4i*>(f + u * mx4_frag_ld(TILES) + mt * MX4_FRAG + fl);
+            hi[i % RING] = *reinterpret_cast<const v2u*>(f + u * mx4_frag_ld(TILES) + mt * MX4_FRAG + fh);
+            if constexpr (!KEEP || u == 0 || (!SHIFT && ((K0 + u) & 3) == 0)) {
+                const int x = *reinterpret_cast<const int*>(sc + (size_t)(((ks0 + (SHIFT ? 0 : u)) >> 2) * TILES + mt) * 256 + sl);
+                xs[KEEP ? mt : i % RING] = SHIFT ? (int)((unsigned)x >> ((ks0 & 3) * 8)) : x;
+            }
         };
         int ys[NB][SW];
 #pragma unroll
@@ -320,7 +324,7 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
             for (int nb = 0; nb < NB; ++nb) {
                 const v8i y = __builtin_shufflevector(b.w[nb][u], b.w[nb][u], 0, 1, 2, 3, -1, -1, -1, -1);
                 const v4f c = FIRST && u == 0 ? (v4f){0.f, 0.f, 0.f, 0.f} : acc[mt][nb];
-                acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 2, 4, kk & 3, xs[i % RING], kk & 3,
+                acc[mt][nb] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 2, 4, kk & 3, xs[KEEP ? mt : i % RING], kk & 3,
                                                                                ys[nb][(kk >> 2) - (K0 >> 2)]);
             }
         });
