@@ -270,13 +270,14 @@ static Mx4Shape mx4_shape(int type, int dim, int mt, bool wide) {
     p.lds = mx4_lds(ks, p.u, mx4_tiles(p.nd, p.mt));
     return p;
 }
-// The shape for nq queries against rows in `spans` pieces of whole units: fewer tiles than the queries fill where the
-// workgroups would not reach all compute units, since a workgroup's first work is to split its queries (32 fp32 queries x 10k x
-// 768: 18.5 us with all of them in each workgroup, 9.5 with eight)
+// The shape for nq queries, where groups_of(shape) workgroups have a whole unit of rows: fewer tiles than the queries fill where
+// these would leave more than half of the compute units idle, since a workgroup's first work is to split its queries (32
+// fp32 queries x 10k x 768: 10.1 us with all of them in each workgroup, 6.8 with sixteen; 64 bf16 queries x 2000 x 1024: 11.0, and
+// 5.2 with eight.  Asked to reach all of them 32 x 40k takes 12.7, like this 11.0)
 template <typename Units>
 static Mx4Shape mx4_shape_for(int type, int dim, long long nq, bool wide, Units groups_of) {
     Mx4Shape p = mx4_shape(type, dim, mx4_tiles_for(type == RAG_MX4_F32 ? 5 : 4, nq), wide);
-    while (p.mt > 1 && groups_of(p) < 256) p = mx4_shape(type, dim, p.mt / 2, wide);
+    while (p.mt > 1 && groups_of(p) < 128) p = mx4_shape(type, dim, p.mt / 2, wide);
     return p;
 }
 constexpr long long MX4_MOST_ROWS = 8192;               // of a piece of a ragged group
@@ -406,7 +407,7 @@ static Mx4Plan mx4_plan(long long n, long long nq, int k) {
 }
 
 // Pieces on their way to the device.  A few KB as a kernel that reads page-locked memory cost a launch; as a copy command they
-// wait for its own signalling (a plan of 591 pieces with the product behind it: 49 us by copy, 32 by kernel).  The
+// wait for its own signalling (a plan of 591 pieces with the product behind it: 47 us by copy, 30 by kernel).  The
 // kernel's last store says that the block may be used again.
 struct Mx4Slot {
     char* host = nullptr;
@@ -619,7 +620,7 @@ int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngro
     *total = sum;
     // rows of a piece: enough pieces to fill the chip several times over, each long enough to pay for staging its queries;
     // with one tile, where that costs little and more workgroups fit a compute unit, shorter ones (1000 groups of 3 fp32
-    // queries x 2000 rows x 384: 106 us in pieces of 2048, 85 of 512)
+    // queries x 2000 rows x 384: 106 us in pieces of 2048, 90 of 512)
     long long part = 0;
     auto queries = [&](long long g) { return (uint32_t)(groups[4 * g + 1] - groups[4 * g]); };
     auto rows = [&](long long g) { return (uint32_t)(groups[4 * g + 3] - groups[4 * g + 2]); };
@@ -641,7 +642,7 @@ int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngro
     *n_items = pieces;
     if (pieces > max_items) return RAG_OK;
     // The longest pieces first, so that the last workgroups to begin are the short ones (200 groups of up to 24 fp16 queries x
-    // 3000 rows x 384: 38 us in the groups' order, 32 like this; 512 lists of 400 rows x 1024: 26.6, 25.8)
+    // 3000 rows x 384: 32.4 us in the groups' order, 28.5 like this; 512 lists of 400 rows x 1024: 24.2, 22.0)
     constexpr int CLASSES = MX4_MOST_ROWS / 16;
     int64_t place[CLASSES] = {};                          // pieces of each (rows - 1) / 16, then where the next one of them goes
     for (long long g = 0; g < ngroups; ++g) {

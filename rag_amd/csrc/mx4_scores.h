@@ -186,16 +186,20 @@ __device__ __forceinline__ float fifth_digits(float v0, float v1, float v2) {
 // matrix unit; nothing but the query fragments goes through LDS, and there is no barrier after they are staged.  The wave's
 // memory operations are the same whatever the data: the fetch ahead is made past the last rows too (of the last ones again), and
 // lanes without a score to store address nothing behind a buffer descriptor's end.  Behind a branch the compiler would have to
-// wait for all of them at every turn, stores too (256 fp32 queries x 200k x 768: 160 us with branches around the stores, 156 without).
+// wait for all of them at every turn, stores too (branches around the stores cost 2.5 % of 256 fp32 queries x 200k x 768).
 //
-// BIG, for stores that no cache keeps: rows are fetched past them (4M x 768, one query: 299 -> 264 us), and where up to 8
+// BIG, for stores that no cache keeps: rows are fetched past them (4M x 768, one query: 303 -> 260 us), and where up to 8
 // queries meet a row a wave takes four tiles of sixteen rows in a row and stores their scores together, 256 contiguous bytes
-// per query instead of 64 (264 -> 255).
+// per query instead of 64 (one query 265 -> 260, eight 320 -> 306).
 //
-// Where it stands.  Few queries: bound by HBM.  4M x 768, one query: 255 us, 6.6 TB/s of rows, scales and scores; reading the same
-// rows alone takes 220 us (7.0 TB/s), and with one 256-byte store per 24 KB 236 to 247.  16 bf16 queries x 1M x 1024: 113 us, 5.4 TB/s
-// (100 without the stores).  Many queries: bound by the matrix unit and the LDS that feeds it (a tile's fragments serve NB row blocks):
-// 256 fp32 queries x 200k x 768: 156 us, 2.5e15 eight-bit operations a second, against 2.8e15 of a large library product of eight-bit matrices.
+// Where it stands.  Few queries: bound by HBM.  4M x 768, one query: 258 us, 6.4 TB/s of rows, scales and scores; reading the same
+// rows alone takes 220 us (7.0 TB/s), and with one 256-byte store per 24 KB 236 to 247.  16 bf16 queries x 1M x 1024: 107 us, 5.7 TB/s.
+// Many queries: 256 fp32 queries x 200k x 768: 128 us, 3.1e15 digit operations a second of the 8.6e15 that the instruction alone
+// reaches; 105 without its stores and with the rows in the nearest cache.  The matrix unit is busy a third of the time and the
+// LDS, whose fragments serve NB row blocks each, for three quarters by its bytes; three or four row blocks to a fragment need
+// more registers than two waves to a SIMD have (four waves a workgroup with four blocks: the same time; half as many queries with
+// two to four blocks: 176 to 180 us), fragments fetched three or four tiles ahead change nothing.  The longest rows
+// lose most: 256 queries x 100k x 4096 546 us, since the fragments of 8 queries are all that the LDS holds.
 template <int ND, int MT, int NB, int U, int NW, int STEPS, bool BIG>
 __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     typedef Mx4Digits<ND, MT> L;
