@@ -42,7 +42,7 @@ struct Mx4ScoreArgs {
     const uint8_t* scales;
     const void* q;
     long long ldq;               // elements
-    int q_type, q_vec, dim, ks, ksu, code_ld, scale_ld, normalize;
+    int q_type, dim, ks, ksu, code_ld, scale_ld, normalize;
     unsigned per;                        // ceil(2^32 / (4 ks)): the query of a group of 32 elements by a multiplication
     size_t code_bytes, scale_bytes;      // of the whole store
     float* out;

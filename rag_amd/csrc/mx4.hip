@@ -318,7 +318,6 @@ static Mx4ScoreArgs mx4_score_args(const rag_mx4_store_t* st, const Mx4Shape& p,
     a.q = q;
     a.ldq = ldq;
     a.q_type = q_type;
-    a.q_vec = mx4_aligned(q, ldq, q_type);
     a.dim = st->dim;
     a.ks = mx4_blocks(st->dim);
     a.per = (unsigned)((0x100000000ull + 4 * a.ks - 1) / (4 * a.ks));

@@ -19,6 +19,9 @@ typedef unsigned v6u __attribute__((ext_vector_type(6)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef float v32f __attribute__((ext_vector_type(32)));
 typedef int v2i __attribute__((ext_vector_type(2)));
+// wide loads from addresses that are only aligned to their elements
+typedef v4i v4i_apart __attribute__((aligned(2)));
+typedef v2i v2i_apart __attribute__((aligned(2)));
 typedef short v2s __attribute__((ext_vector_type(2)));
 
 template <int N, typename F>

@@ -40,13 +40,13 @@ template <int ND, int MT, int EL>
 __device__ __forceinline__ void mx4_stage_unit(const Mx4ScoreArgs& a, const char* q, int u, uint8_t* frag, uint8_t* sc) {
     typedef Mx4Digits<ND, MT> L;
     constexpr int QPT = L::QPT, TILES = L::TILES, ESIZE = ND == 5 ? 4 : 2, SHARE = 32 / EL;
-    typedef typename std::conditional<EL * ESIZE % 16 == 0, v4i, v2i>::type Raw;
+    typedef typename std::conditional<EL * ESIZE % 16 == 0, v4i_apart, v2i_apart>::type Raw;
     constexpr int PIECES = EL * ESIZE / sizeof(Raw), DW = sizeof(Raw) / 4;
     // s: the query; its group of 32 elements; the lane's part `in` of that
     const int ug = u / SHARE, in = u % SHARE, s = (int)__umulhi((unsigned)ug, a.per), group = ug - s * a.ks * 4, at0 = group * 32 + in * EL;
     const char* row = q + (size_t)s * a.ldq * ESIZE;
     float v[EL];
-    if (a.q_vec && at0 + EL <= a.dim) {
+    if (at0 + EL <= a.dim) {
         Raw raw[PIECES];
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) raw[j] = reinterpret_cast<const Raw*>(row + (size_t)at0 * ESIZE)[j];
@@ -58,9 +58,17 @@ __device__ __forceinline__ void mx4_stage_unit(const Mx4ScoreArgs& a, const char
                 v[j] = a.q_type == RAG_MX4_BF16 ? bf16_f32(h) : f16_f32((unsigned short)h);
             }
         }
-    } else {                                                    // unaligned, or the end of a row: zeros behind it
+    } else {                                                    // the end of a row: zeros behind it
+        typedef typename std::conditional<ND == 5, float, unsigned short>::type Elem;
+        Elem raw[EL];
 #pragma unroll
-        for (int j = 0; j < EL; ++j) v[j] = at0 + j < a.dim ? mx4_elem(row, a.q_type, at0 + j) : 0.f;
+        for (int j = 0; j < EL; ++j) raw[j] = reinterpret_cast<const Elem*>(row)[at0 + j < a.dim ? at0 + j : a.dim - 1];
+#pragma unroll
+        for (int j = 0; j < EL; ++j) {
+            if constexpr (ND == 5) v[j] = raw[j];
+            else v[j] = a.q_type == RAG_MX4_BF16 ? bf16_f32(raw[j]) : f16_f32(raw[j]);
+            v[j] = at0 + j < a.dim ? v[j] : 0.f;
+        }
     }
     unsigned most = 0;
 #pragma unroll

@@ -239,6 +239,26 @@ def test_scores(nq, n, dim, dtype):
     assert np.array_equal(index.scores(q, b, e).cpu().numpy(), got[:, b:e])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [31, 100, 257, 384, 500, 640, 768, 900, 1000, 1024, 1100, 1536, 2048, 4096, 8192])
+def test_many_queries_against_many_rows(dim, dtype):
+    """Rows enough for the kernels that take 8, 16 and 32 queries at a time, for every number of blocks: the scores are those that
+    the kernels for few queries give the same rows, bit for bit."""
+    import torch
+    from rag_amd import QuantizedIndex
+    rng = np.random.default_rng(dim)
+    small, v = _index(rng, 256, dim)
+    codes, scales = small.packed()
+    at = torch.from_numpy(rng.integers(0, 256, 40_001)).cuda()
+    index = QuantizedIndex.from_packed(codes[at], scales[at], dim)
+    for nq, first in ((7, 0), (16, 0), (37, 0), (37, 1)):               # first 1: rows that start between the elements of a wide load
+        wide, wide64 = _rows(rng, nq, dim + first, dtype)
+        q, q64 = wide[:, first:], wide64[:, first:]
+        part = torch.cat([small.scores(q[i:i + 1]) for i in range(nq)])
+        _check_scores(part.cpu().numpy(), q64, v, dtype)
+        assert torch.equal(index.scores(q), part[:, at]), (nq, first)
+
+
 def test_the_average_error_of_a_score_is_that_of_fp32():
     """Root mean square: independent roundings of half a step at most, spread evenly (2^-24 / sqrt(3)) over 8 partial sums per
     block and 4 digit sums, of the sum of |products|; a plain fp32 product is allowed the same."""
