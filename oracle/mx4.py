@@ -53,22 +53,18 @@ def scores(q, v):
     return np.asarray(q, np.float64) @ np.asarray(v, np.float64).T
 
 
-def score_bound(q, v, digits):
-    """A bound of |computed - exact| for every score.  Queries enter the product as `digits` base-32 digits relative to the
-    power of two of their group's largest element: what is cut off, times |v|, is lost.  Then every block of 128 elements adds at
-    most 8 partial sums to a running fp32 sum per digit and the digits are added in 4 steps: each a rounding of at
-    most half a step (2^-24) of at most the sum of |products|, to which the digits behind the first add a 16th each time."""
-    q = np.asarray(q, np.float64)
-    nq, dim = q.shape
-    g = (dim + 31) // 32
-    p = np.zeros((nq, g * 32))
-    p[:, :dim] = q
-    p = p.reshape(nq, g, 32)
-    a = np.abs(p).max(2)
-    e = np.maximum(np.frexp(a)[1] - 1 - 3, -100)
-    unit = np.exp2(e.astype(np.float64) - 5 * (digits - 1))[:, :, None]
-    cut = np.abs(p - np.rint(p / unit) * unit).reshape(nq, g * 32)[:, :dim]
-    blocks = (dim + 127) // 128
-    av = np.abs(np.asarray(v, np.float64))
-    size = np.abs(q) @ av.T * (16.0 / 15.0)
-    return cut @ av.T + (8 * blocks + 4) * 2.0 ** -24 * size
+def product_bound(q, v):
+    """A bound of |computed - exact| for every score, from the definition alone: queries and values are taken as they are, a score
+    is the sum of their products in fp32 in any order.  Products with a zero add nothing; the others are added with one rounding
+    each, of at most half a step (2^-24) of at most the sum of |products|, and so are up to four partial sums."""
+    q, v = np.abs(np.asarray(q, np.float64)), np.abs(np.asarray(v, np.float64))
+    terms = (q > 0).astype(np.float64) @ (v > 0).astype(np.float64).T
+    return (terms + 4) * 2.0 ** -24 * (q @ v.T)
+
+
+def score_bound(q, v, digits=None):
+    """A bound of |computed - exact| for every score, tighter than product_bound for long rows: per block of 128 elements eight
+    roundings of half a step (2^-24) of the sum of |products|, and four for the partial sums.  Nothing is allowed for the operands,
+    which enter the product whole (``digits`` once said how much of a query did, and is not used)."""
+    blocks = (np.asarray(q).shape[1] + 127) // 128
+    return (8 * blocks + 4) * 2.0 ** -24 * (np.abs(np.asarray(q, np.float64)) @ np.abs(np.asarray(v, np.float64)).T)

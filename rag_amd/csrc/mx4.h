@@ -20,10 +20,7 @@ __host__ __device__ __forceinline__ size_t mx4_code_at(long long row, int code_l
 }
 __host__ __device__ __forceinline__ int mx4_scale_at(int group) { return (group >> 4) * 16 + (group & 3) * 4 + ((group >> 2) & 3); }
 
-constexpr int MX4_MAX_DIM = 8192;          // the query fragments of one matrix tile (2 KiB per block of 128) fit the LDS
-
-constexpr int MX4_FRAG = 1536;             // a block of one tile of query digits: 64 lanes of 32 six-bit values
-__host__ __device__ constexpr int mx4_frag_ld(int tiles) { return tiles * MX4_FRAG + 64; }     // from block to block
+constexpr int MX4_MAX_DIM = 8192;          // eight rows of query parts (2 KiB per block of 128) fit the LDS
 
 // One piece of the grouped product: `nq` queries from q0 against `rows` rows from row0; score (i, r) goes to
 // out[at + i * ld + r].  Written by rag_mx4_plan_groups, read by the kernel.
@@ -42,8 +39,8 @@ struct Mx4ScoreArgs {
     const uint8_t* scales;
     const void* q;
     long long ldq;               // elements
-    int q_type, dim, ks, ksu, code_ld, scale_ld, normalize;
-    unsigned per;                        // ceil(2^32 / (4 ks)): the query of a group of 32 elements by a multiplication
+    int dim, ks, ksu, code_ld, scale_ld, normalize;
+    unsigned per;                        // ceil(2^32 / (16 ks)): the query of a unit of 8 elements by a multiplication
     size_t code_bytes, scale_bytes;      // of the whole store
     float* out;
     // grouped: one workgroup per item
@@ -54,13 +51,16 @@ struct Mx4ScoreArgs {
     int nq, nqb;
 };
 
-// Which kernel a product takes: from the queries that meet a row, and the row's length.
+// Which kernel a product takes (mx4_scores.h): from the queries that meet a row, and the row's length.
 struct Mx4Shape {
-    int nd, mt, nb, u, nw, steps, ksu, qb;
+    bool many;                   // the kernel for many queries; else the one for few
+    int qpt, mt, nb, r, u, nw, steps, ksu;
+    int qb;                      // queries of a workgroup
     bool big;
     size_t lds;
 };
 int mx4_launch_f32(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s);      // mx4_scores_f32.hip
-int mx4_launch_16(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s);       // mx4_scores_16.hip
+int mx4_launch_bf16(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s);     // mx4_scores_bf16.hip
+int mx4_launch_f16(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s);      // mx4_scores_f16.hip
 
 }  // namespace rag

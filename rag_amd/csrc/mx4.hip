@@ -240,52 +240,94 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(Mx4ReadArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ products (kernels: mx4_scores.h)
-static int mx4_tiles(int nd, int mt) { return nd == 5 && mt > 1 ? mt + (mt + 3) / 4 : mt; }        // Mx4Digits::TILES
-static size_t mx4_lds(int ks, int u, int tiles) {
-    const int ksu = (ks + u - 1) / u * u;
-    return (size_t)ksu * mx4_frag_ld(tiles) + (size_t)(ksu + 3) / 4 * tiles * 256 + (size_t)tiles * 4 * sizeof(float);
+constexpr long long MX4_MOST_ROWS = 8192;               // of a piece of a ragged group
+constexpr long long MX4_WIDE = 40 * 1000 * 1000;         // 12 * 4 bytes * this, and a tile, stay below 2^31
+
+// The shapes of a type, by the queries of a workgroup: those of the kernel for few queries, then those of the one for many.  32 of
+// a type's queries and more go to the latter, whose fragments serve several row blocks; fp32 queries from 9 on, three of whose tiles would
+// take as many LDS reads as there are there (16 x 4M x 768: 405 us)
+struct Mx4Level {
+    int qpt, mt, nb;             // nb 0: the kernel for few queries
+};
+struct Mx4Levels {
+    int count, half;             // half: the level of one full tile, half of which is taken where the LDS does not hold it
+    Mx4Level of[5];
+};
+static const Mx4Levels& mx4_levels(int type) {
+    static const Mx4Levels f32 = {4, 0, {{4, 1, 0}, {4, 2, 0}, {16, 3, 2}, {16, 6, 3}}};                      // 4, 8, 16, 32 queries
+    static const Mx4Levels f16 = {4, 1, {{4, 1, 0}, {8, 1, 0}, {8, 2, 0}, {8, 4, 4}}};                        // 4, 8, 16, 32
+    static const Mx4Levels bf16 = {5, 2, {{4, 1, 0}, {8, 1, 0}, {16, 1, 0}, {16, 2, 0}, {16, 4, 4}}};         // 4, 8, 16, 32, 64
+    return type == RAG_MX4_F32 ? f32 : type == RAG_MX4_F16 ? f16 : bf16;
 }
-// tiles that nq queries fill
-static int mx4_tiles_for(int nd, long long nq) { return nq <= (nd == 5 ? 3 : 4) ? 1 : nq <= 8 ? 2 : nq <= 16 ? 4 : 8; }
-// mt: most tiles.  wide: the scores of two queries may lie further apart than a lane's 32-bit offset reaches (LONG kernels have none)
-static Mx4Shape mx4_shape(int type, int dim, int mt, bool wide) {
-    Mx4Shape p = {};
+static int mx4_most(int type, int level) {
+    const Mx4Level& v = mx4_levels(type).of[level];
+    return type == RAG_MX4_F32 && v.qpt == 16 ? v.mt / 3 * 16 : v.mt * v.qpt;
+}
+// lowest level whose workgroups take nq queries (or the last one)
+static int mx4_level_for(int type, long long nq) {
+    int level = 0;
+    while (level + 1 < mx4_levels(type).count && mx4_most(type, level) < nq) ++level;
+    return level;
+}
+// The shape of a level, or of the next lower one that there is for rows of this length.  wide: the scores of two queries may lie
+// further apart than a lane's 32-bit offset reaches (the kernel for up to 8 queries of a large store has a base for each)
+static Mx4Shape mx4_shape(int type, int dim, int level, bool wide) {
+    constexpr int LDS = 160 * 1024;
     const int ks = mx4_blocks(dim);
-    p.nd = type == RAG_MX4_F32 ? 5 : 4;
-    // rows of up to 8 blocks: one fetch, or two of half the row where more tiles need the registers
-    auto fetch = [&](int m, int* steps) {
-        *steps = m <= 2 ? ks <= 8 && ks != 5 && ks != 7 : ks == 3 ? 1 : ks == 4 || ks == 6 || (ks == 8 && m == 4) ? 2 : 0;
-        if (*steps) return ks / *steps;
-        if (m <= 2) return (ks & 7) == 0 || (ks & 7) > 4 ? 8 : 4;       // (blocks past the row's are fetched again, from the caches)
-        return m == 4 && (ks & 3) == 0 ? 4 : (ks & 1) == 0 ? 2 : 1;
-    };
-    p.mt = wide ? std::min(mt, 2) : mt;
-    while (p.mt > 1 && mx4_lds(ks, fetch(p.mt, &p.steps), mx4_tiles(p.nd, p.mt)) > 160 * 1024) p.mt /= 2;
-    p.u = fetch(p.mt, &p.steps);
-    p.big = wide;
-    p.nb = p.mt <= 4 ? 1 : 2;
-    p.nw = p.mt >= 4 || p.steps == 0 ? 8 : 4;           // eight waves share the fragments where these fill much of the LDS
-    p.ksu = (ks + p.u - 1) / p.u * p.u;
-    p.qb = p.nd == 5 && p.mt == 1 ? 3 : 4 * p.mt;
-    p.lds = mx4_lds(ks, p.u, mx4_tiles(p.nd, p.mt));
-    return p;
+    Mx4Shape p = {};
+    for (;; --level) {
+        const Mx4Level& v = mx4_levels(type).of[level];
+        p.qpt = v.qpt;
+        p.mt = v.mt;
+        p.nb = v.nb;
+        p.qb = mx4_most(type, level);
+        p.many = v.nb > 0;
+        p.r = 16;
+        if (wide && (p.many || p.qb > 8)) continue;
+        if (p.many) {
+            p.nw = 8;
+            p.ksu = ks;
+            p.lds = (size_t)ks * p.mt * 4096 + p.qb * sizeof(float);
+            p.steps = p.lds <= LDS;                          // the whole queries lie in LDS; else two blocks of them
+            if (!p.steps) p.lds = (size_t)2 * p.mt * 4096 + p.qb * sizeof(float);
+            return p;
+        }
+        p.big = wide;
+        p.nb = 1;
+        p.steps = ks <= 8 && ks != 5 && ks != 7;
+        p.u = p.steps ? ks : (ks & 7) == 0 || (ks & 7) > 4 ? 8 : 4;      // (blocks past the row's are fetched again, from the caches)
+        p.nw = p.steps ? 4 : 8;                              // eight waves share the fragments where these fill much of the LDS
+        p.ksu = (ks + p.u - 1) / p.u * p.u;
+        const size_t inv = (size_t)p.qb * sizeof(float);
+        p.lds = (size_t)p.ksu * p.mt * 4096 + inv;
+        if (p.lds <= LDS) return p;
+        if (level > 0) continue;
+        // the longest rows: one tile of which the LDS holds eight rows
+        const Mx4Level& one = mx4_levels(type).of[mx4_levels(type).half];
+        p.qpt = one.qpt;
+        p.r = 8;
+        p.u = 8;
+        p.ksu = (ks + 7) / 8 * 8;
+        p.lds = (size_t)p.ksu * 2048 + one.qpt * sizeof(float);
+        p.qb = one.qpt / 2;
+        return p;
+    }
 }
-// The shape for nq queries, where groups_of(shape) workgroups have a whole unit of rows: fewer tiles than the queries fill where
-// these would leave more than half of the compute units idle, since a workgroup's first work is to split its queries (32
-// fp32 queries x 10k x 768: 10.1 us with all of them in each workgroup, 6.8 with sixteen; 64 bf16 queries x 2000 x 1024: 11.0, and
-// 5.2 with eight.  Asked to reach all of them 32 x 40k takes 12.7, like this 11.0)
+// The shape for nq queries, where groups_of(shape) workgroups have a whole unit of rows: fewer queries to a workgroup where more would
+// leave more than half of the compute units idle (32 fp32 queries x 10k x 768: 7.8 us, asked to fill a quarter of them 9.3; x 40k 14.6, 17.0;
+// 64 bf16 queries x 2000 x 1024: 5.6, 7.8)
 template <typename Units>
 static Mx4Shape mx4_shape_for(int type, int dim, long long nq, bool wide, Units groups_of) {
-    Mx4Shape p = mx4_shape(type, dim, mx4_tiles_for(type == RAG_MX4_F32 ? 5 : 4, nq), wide);
-    while (p.mt > 1 && groups_of(p) < 128) p = mx4_shape(type, dim, p.mt / 2, wide);
+    int level = mx4_level_for(type, nq);
+    Mx4Shape p = mx4_shape(type, dim, level, wide);
+    while (level > 0 && groups_of(p) < 128) p = mx4_shape(type, dim, --level, wide);
     return p;
 }
-constexpr long long MX4_MOST_ROWS = 8192;               // of a piece of a ragged group
-constexpr long long MX4_WIDE = 100 * 1000 * 1000;        // 3 * 4 bytes * this, and a tile, stay below 2^31
 
-static int mx4_launch_any(const Mx4Shape& p, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s) {
+static int mx4_launch_any(const Mx4Shape& p, int type, const Mx4ScoreArgs& a, long long grid, int device, hipStream_t s) {
     if (grid < 1 || grid * p.nw * 64 > 0xffffffffLL) return fail(RAG_ERR_INVALID, "four-bit product: grid out of range");
-    return p.nd == 5 ? mx4_launch_f32(p, a, grid, device, s) : mx4_launch_16(p, a, grid, device, s);
+    return type == RAG_MX4_F32 ? mx4_launch_f32(p, a, grid, device, s) : type == RAG_MX4_F16 ? mx4_launch_f16(p, a, grid, device, s)
+                                                                                          : mx4_launch_bf16(p, a, grid, device, s);
 }
 
 static bool mx4_lies_on(const void* p, size_t boundary) { return (reinterpret_cast<uintptr_t>(p) & (boundary - 1)) == 0; }
@@ -311,16 +353,15 @@ static int mx4_rows_per_block(long long count, int upr) {
     const long long full = std::max(1, std::min(MX4_ROWS, 256 * MX4_UNITS / upr));
     return (int)std::max<long long>(1, std::min<long long>(full, count / 512));
 }
-static Mx4ScoreArgs mx4_score_args(const rag_mx4_store_t* st, const Mx4Shape& p, const void* q, int q_type, long long ldq, int normalize, float* out) {
+static Mx4ScoreArgs mx4_score_args(const rag_mx4_store_t* st, const Mx4Shape& p, const void* q, long long ldq, int normalize, float* out) {
     Mx4ScoreArgs a = {};
     a.codes = static_cast<const uint8_t*>(st->codes);
     a.scales = static_cast<const uint8_t*>(st->scales);
     a.q = q;
     a.ldq = ldq;
-    a.q_type = q_type;
     a.dim = st->dim;
     a.ks = mx4_blocks(st->dim);
-    a.per = (unsigned)((0x100000000ull + 4 * a.ks - 1) / (4 * a.ks));
+    a.per = (unsigned)((0x100000000ull + 16 * a.ks - 1) / (16 * a.ks));
     a.ksu = p.ksu;
     a.code_ld = mx4_code_bytes(st->dim);
     a.scale_ld = mx4_scale_bytes(st->dim);
@@ -337,11 +378,10 @@ static int mx4_scores(const rag_mx4_store_t* st, long long row0, long long rows,
     Mx4Shape p = mx4_shape_for(q_type, st->dim, nq, out_ld > MX4_WIDE, [&](const Mx4Shape& s) {
         return (rows + 16LL * s.nb * s.nw - 1) / (16LL * s.nb * s.nw) * ((nq + s.qb - 1) / s.qb);
     });
-    Mx4ScoreArgs a = mx4_score_args(st, p, q, q_type, ldq, normalize, out);
-    // Past the caches once the rows exceed the 256 MB that they keep from call to call (400k x 768, 167 MB, one query: 27 us kept, 31
-    // past them; 800k: 61 and 59), and for up to 8 queries, whose waves then take 64 rows at a time, once these keep the waves busy
-    // (50k x 4096: 35 us in pieces of 64 rows, 21 of 16)
-    p.big = p.big || (nq <= p.qb && rows * (a.code_ld + a.scale_ld) > 256LL << 20 && (p.mt > 2 || rows >= 64 * 4096));
+    Mx4ScoreArgs a = mx4_score_args(st, p, q, ldq, normalize, out);
+    // Past the caches once the rows exceed the 256 MB that they keep from call to call, and for up to 8 queries, whose waves then
+    // take 64 rows at a time, once these keep the waves busy
+    p.big = p.big || (!p.many && nq <= p.qb && rows * (a.code_ld + a.scale_ld) > 256LL << 20 && (p.qb > 8 || rows >= 64 * 4096));
     a.row0 = row0;
     a.rows = rows;
     a.out_ld = out_ld;
@@ -349,18 +389,19 @@ static int mx4_scores(const rag_mx4_store_t* st, long long row0, long long rows,
     a.nqb = (int)((nq + p.qb - 1) / p.qb);
     const long long unit = 16LL * p.nb * p.nw;                  // rows of one step of a workgroup
     const long long units = (rows + unit - 1) / unit;
-    if (a.nqb == 1) return mx4_launch_any(p, a, std::min<long long>(units, p.mt == 8 ? 256 : p.nw == 8 ? 512 : 1024), st->device, s);
+    // workgroups that are at work at a time
+    const long long seats = 256LL * (p.many ? 1 : std::max<long long>(1, std::min<long long>(16 / p.nw, 160 * 1024 / p.lds)));
+    if (!p.many && a.nqb == 1) return mx4_launch_any(p, q_type, a, std::min(units, seats), st->device, s);
     // Slabs: as many as make the workgroups come out even over the chip's compute units, each long against the staging of
     // its queries (about two units of work)
-    const long long seats = 256LL * (p.mt == 8 ? 1 : 2);
     long long best = 1, least = LLONG_MAX;
     for (long long n = 1; n <= std::min<long long>(units, std::max<long long>(64, 8 * seats / a.nqb)); ++n) {
-        const long long cost = (n * a.nqb + seats - 1) / seats * ((units + n - 1) / n + 2);
+        const long long cost = (n * a.nqb + seats - 1) / seats * ((units + n - 1) / n + (p.many ? 1 : 2));
         if (cost < least) { least = cost; best = n; }
     }
     a.slab = (units + best - 1) / best * unit;
     a.slabs = (rows + a.slab - 1) / a.slab;
-    return mx4_launch_any(p, a, (a.slabs * a.nqb + 7) / 8 * 8, st->device, s);
+    return mx4_launch_any(p, q_type, a, (a.slabs * a.nqb + 7) / 8 * 8, st->device, s);
 }
 
 int direct_select_segments(long long nq, long long n_row, long long seg_rows, int k, float min_score, const uint8_t* mask,
@@ -629,7 +670,7 @@ int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngro
         long long work = 0, items = 0;
         for (long long g = 0; g < ngroups; ++g)
             work += (long long)parts(queries(g), s.qb) * rows(g);
-        part = std::max<long long>(4 * unit, std::min<long long>(MX4_MOST_ROWS, (work / (s.mt == 1 ? 4096 : 1024) + unit - 1) / unit * unit));
+        part = std::max<long long>(4 * unit, std::min<long long>(MX4_MOST_ROWS, (work / (!s.many && s.mt == 1 ? 4096 : 1024) + unit - 1) / unit * unit));
         for (long long g = 0; g < ngroups; ++g)
             items += (long long)parts(queries(g), s.qb) * parts(rows(g), (uint32_t)part);
         return items;
@@ -717,14 +758,14 @@ int rag_mx4_scores_grouped_device(const rag_mx4_store_t* st, int64_t nq, const v
     if (widest < 1 || widest > nq) return fail(RAG_ERR_INVALID, "widest is not what rag_mx4_plan_groups gave for these queries");
     Mx4DeviceGuard g(st->device);
     if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
-    const Mx4Shape p = mx4_shape(q_type, st->dim, mx4_tiles_for(q_type == RAG_MX4_F32 ? 5 : 4, widest), total > MX4_WIDE);
-    Mx4ScoreArgs a = mx4_score_args(st, p, q_dev, q_type, q_stride, normalize ? 1 : 0, out_dev);
+    const Mx4Shape p = mx4_shape(q_type, st->dim, mx4_level_for(q_type, widest), total > MX4_WIDE);
+    Mx4ScoreArgs a = mx4_score_args(st, p, q_dev, q_stride, normalize ? 1 : 0, out_dev);
     a.nq = (int)nq;
     a.rows = st->n;
     a.total = total;
     for (int64_t i = 0; i < n_items; i += MX4_GRID) {
         a.items = static_cast<const Mx4Item*>(items_dev) + i;
-        if (int rc = mx4_launch_any(p, a, std::min<int64_t>(MX4_GRID, n_items - i), st->device, static_cast<hipStream_t>(stream))) return rc;
+        if (int rc = mx4_launch_any(p, q_type, a, std::min<int64_t>(MX4_GRID, n_items - i), st->device, static_cast<hipStream_t>(stream))) return rc;
     }
     return RAG_OK;
 }

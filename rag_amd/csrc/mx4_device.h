@@ -11,18 +11,12 @@
 namespace rag {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
-typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
-typedef unsigned v6u __attribute__((ext_vector_type(6)));
-typedef float v16f __attribute__((ext_vector_type(16)));
-typedef float v32f __attribute__((ext_vector_type(32)));
-typedef int v2i __attribute__((ext_vector_type(2)));
-// wide loads from addresses that are only aligned to their elements
-typedef v4i v4i_apart __attribute__((aligned(2)));
-typedef v2i v2i_apart __attribute__((aligned(2)));
-typedef short v2s __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef v4i v4i_apart __attribute__((aligned(2)));               // wide loads from addresses that are only aligned to their elements
 
 template <int N, typename F>
 __device__ __forceinline__ void static_for(F f) {
@@ -72,14 +66,10 @@ __device__ __forceinline__ void mx4_load8(const void* row, int i, int dim, float
 }
 
 __device__ __forceinline__ unsigned dpp_max_u32(unsigned v, unsigned o) { return v > o ? v : o; }
-// the largest of |v| (as ordered bits) over each aligned group of 4 / 8 lanes
+// the largest of |v| (as ordered bits) over each aligned group of 4 lanes
 __device__ __forceinline__ unsigned quad_max(unsigned v) {
     v = dpp_max_u32(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
     return dpp_max_u32(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
-}
-__device__ __forceinline__ unsigned oct_max(unsigned v) {
-    v = quad_max(v);
-    return dpp_max_u32(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));   // row_half_mirror
 }
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll

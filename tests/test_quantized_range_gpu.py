@@ -1,0 +1,149 @@
+"""rag_amd.QuantizedIndex over the whole range of its operands: every bit of a query counts, whatever else its group holds,
+and cosine scores hold for vectors of any norm.  Against float64; bounds come from the definition (oracle/mx4.py, product_bound)."""
+import numpy as np
+import pytest
+
+from oracle import mx4
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ["float32", "bfloat16", "float16"]
+
+
+def _t(name):
+    import torch
+    return getattr(torch, name)
+
+
+def _unit_rows(dim, n):
+    """An index whose row r holds a one at element r % dim and zeros elsewhere: its scores are the queries' elements."""
+    import torch
+    from rag_amd import QuantizedIndex
+    g = (dim + 31) // 32
+    codes = np.zeros((dim, 16 * g), np.uint8)
+    i = np.arange(dim)
+    codes[i, i // 2] = 2 << (4 * (i % 2))
+    at = torch.arange(n, device="cuda") % dim
+    return QuantizedIndex.from_packed(torch.from_numpy(codes).cuda()[at], torch.full((n, g), 127, dtype=torch.uint8, device="cuda"), dim), at
+
+
+def _any_bits(rng, shape, dtype):
+    """Finite values of the type with any exponent, subnormal ones and zeros among them, as a CUDA tensor."""
+    import torch
+    if dtype == "float32":
+        bits = rng.integers(0, 2 ** 32, shape, dtype=np.uint32)
+        x = torch.from_numpy(bits.view(np.int32)).view(torch.float32)
+    else:
+        bits = rng.integers(0, 2 ** 16, shape, dtype=np.uint16)
+        x = torch.from_numpy(bits.view(np.int16)).view(_t(dtype))
+    return torch.where(torch.isfinite(x), x, torch.ones_like(x)).cuda()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,n", [(32, 32), (45, 3000), (128, 128), (384, 40_001), (640, 700), (768, 30_000), (900, 2000), (1024, 20_000), (1500, 9000),
+                                   (2048, 4096), (4096, 20_000), (5000, 10_001), (8192, 8192)])
+def test_scores_of_unit_rows_are_the_queries(dim, n, dtype):
+    """One product per score: it is the query's element, to the last bit, beside elements of any size."""
+    import torch
+    rng = np.random.default_rng(dim)
+    index, at = _unit_rows(dim, n)
+    for nq in (1, 2, 4, 5, 7, 16, 17, 33, 70):
+        q = _any_bits(rng, (nq, dim), dtype)
+        if nq > 1:
+            q[0] = torch.tensor(1e-2, dtype=q.dtype)
+            q[0, ::32] = torch.tensor(60000.0, dtype=q.dtype)
+            q[1] = torch.randn(dim, device="cuda").to(q.dtype)
+            q[1, 5::32] *= 3000
+        got = index.scores(q)
+        want = q.float()[:, at]
+        assert torch.equal(got, want), (nq, int((got != want).sum()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,nq,n", [(32, 1, 500), (64, 3, 5000), (100, 8, 700), (384, 40, 20_000), (768, 5, 3000), (2048, 20, 2000)])
+@pytest.mark.parametrize("outlier", [30.0, 300.0, 3000.0])
+def test_outliers_that_meet_zeros(dim, nq, n, dtype, outlier):
+    """One large element in every group of a query, where most rows hold a zero: the rest of the group counts in full."""
+    import torch
+    from rag_amd import QuantizedIndex
+    rng = np.random.default_rng(dim + int(outlier))
+    x = rng.standard_normal((min(n, 700), dim))
+    place = rng.integers(0, 32, (dim + 31) // 32) + np.arange(0, dim, 32)
+    place = place[place < dim]
+    x[:, place] = np.where(rng.random((len(x), 1)) < 0.9, 0.0, x[:, place])
+    codes, scales = mx4.quantise(x)
+    v = mx4.values(codes, scales, dim)
+    at = rng.integers(0, len(x), n)
+    index = QuantizedIndex.from_packed(codes[at], scales[at], dim)
+    q = rng.standard_normal((nq, dim))
+    q[:, place] = outlier * np.where(rng.random((nq, len(place))) < 0.5, -1, 1)
+    q = torch.from_numpy(q.astype(np.float32)).to(_t(dtype)).cuda()
+    q64 = q.double().cpu().numpy()
+    got = index.scores(q).cpu().numpy()
+    bound = mx4.product_bound(q64, v)[:, at]
+    assert (np.abs(got - mx4.scores(q64, v)[:, at]) <= bound).all()
+
+
+def _spread(rng, dim, n):
+    """A small index, and a long one of its rows in a random order."""
+    import torch
+    from rag_amd import QuantizedIndex
+    codes, scales = mx4.quantise(rng.standard_normal((256, dim)) * np.exp2(rng.integers(-3, 4, (256, 1))))
+    small = QuantizedIndex.from_packed(codes, scales, dim)
+    codes, scales = small.packed()
+    at = torch.from_numpy(rng.integers(0, 256, n)).cuda()
+    return small, QuantizedIndex.from_packed(codes[at], scales[at], dim), at, mx4.values(codes.cpu().numpy(), scales.cpu().numpy(), dim)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [31, 100, 257, 640, 768, 900, 1300, 2048, 4096, 8192])
+def test_large_batches_have_the_scores_of_single_queries(dim, dtype):
+    """Batches and rows enough for the kernels that take the most queries at a time, with rows whole in LDS and in parts."""
+    import torch
+    rng = np.random.default_rng(dim + 7)
+    small, index, at, v = _spread(rng, dim, 30_011)
+    for nq, first in ((130, 0), (193, 1)):
+        wide = torch.from_numpy((rng.standard_normal((nq, dim + first)) * np.exp2(rng.integers(-9, 9, (nq, dim + first)))).astype(np.float32))
+        q = wide.to(_t(dtype)).cuda()[:, first:]
+        part = torch.cat([small.scores(q[i:i + 1]) for i in range(nq)])
+        q64 = q.double().cpu().numpy()
+        assert (np.abs(part.cpu().numpy() - mx4.scores(q64, v)) <= mx4.product_bound(q64, v)).all()
+        assert torch.equal(index.scores(q), part[:, at])
+        assert torch.equal(index.scores(q, 5, 29_990), part[:, at[5:29_990]])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [96, 768, 1300])
+def test_groups_of_many_queries_have_the_same_scores(dim, dtype):
+    import torch
+    rng = np.random.default_rng(dim + 8)
+    small, index, at, _ = _spread(rng, dim, 20_000)
+    q = torch.from_numpy(rng.standard_normal((150, dim)).astype(np.float32)).to(_t(dtype)).cuda()
+    part = torch.cat([small.scores(q[i:i + 1]) for i in range(150)])
+    for most in (7, 16, 33, 90):
+        a, b = rng.integers(0, 140, 200), rng.integers(0, 19_000, 200)
+        groups = np.stack([a, np.minimum(150, a + rng.integers(0, most + 1, 200)), b, np.minimum(20_000, b + rng.integers(0, 1500, 200))], 1)
+        plan = index.plan_groups(groups, 150, q.dtype)
+        for got, (q0, q1, r0, r1) in zip(plan.split(index.scores_grouped(q, plan)), groups):
+            assert torch.equal(got, part[q0:q1][:, at[r0:r1]])
+
+
+def test_queries_beyond_the_range_of_their_type_are_nan():
+    """An infinity or a NaN makes every score of its query NaN, and of no other; the largest finite numbers are finite."""
+    import torch
+    rng = np.random.default_rng(3)
+    for n in (64, 40_000):
+        index, at = _unit_rows(96, n)
+        for dtype in TYPES:
+            for nq in (3, 40, 130):
+                q = _any_bits(rng, (nq, 96), dtype)
+                q[2] = torch.finfo(q.dtype).max * torch.from_numpy(rng.choice([-1.0, 1.0], 96)).cuda()
+                clean = index.scores(q)
+                assert torch.equal(clean, q.float()[:, at])
+                for bad in (np.inf, -np.inf, np.nan):
+                    p = q.clone()
+                    p[1, 70] = bad
+                    got = index.scores(p)
+                    assert torch.isnan(got[1]).all()
+                    got[1] = clean[1]
+                    assert torch.equal(got, clean)
