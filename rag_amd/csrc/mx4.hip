@@ -100,8 +100,9 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
     }
     if (a.normalize) {
         for (int r = tid >> 6; r < nr; r += 4) {
-            const float inv = wave_inv_norm(x + (size_t)r * a.ldx * ESIZE, TYPE, a.dim, lane);
-            if (lane == 0) s_inv[r] = inv;
+            int k;
+            const float inv = wave_inv_norm(x + (size_t)r * a.ldx * ESIZE, TYPE, a.dim, lane, k);
+            if (lane == 0) s_inv[r] = inv == inv ? fminf(ldexpf(inv, k), FLT_MAX) : inv;
         }
         __syncthreads();
     }
@@ -287,9 +288,10 @@ static Mx4Shape mx4_shape(int type, int dim, int level, bool wide) {
         if (p.many) {
             p.nw = 8;
             p.ksu = ks;
-            p.lds = (size_t)ks * p.mt * 4096 + p.qb * sizeof(float);
+            const size_t factors = (size_t)p.qb * 8;
+            p.lds = (size_t)ks * p.mt * 4096 + factors;
             p.steps = p.lds <= LDS;                          // the whole queries lie in LDS; else two blocks of them
-            if (!p.steps) p.lds = (size_t)2 * p.mt * 4096 + p.qb * sizeof(float);
+            if (!p.steps) p.lds = (size_t)2 * p.mt * 4096 + factors;
             return p;
         }
         p.big = wide;
@@ -298,8 +300,7 @@ static Mx4Shape mx4_shape(int type, int dim, int level, bool wide) {
         p.u = p.steps ? ks : (ks & 7) == 0 || (ks & 7) > 4 ? 8 : 4;      // (blocks past the row's are fetched again, from the caches)
         p.nw = p.steps ? 4 : 8;                              // eight waves share the fragments where these fill much of the LDS
         p.ksu = (ks + p.u - 1) / p.u * p.u;
-        const size_t inv = (size_t)p.qb * sizeof(float);
-        p.lds = (size_t)p.ksu * p.mt * 4096 + inv;
+        p.lds = (size_t)p.ksu * p.mt * 4096 + (size_t)p.qb * 8;      // (with a factor and a power of two for each query)
         if (p.lds <= LDS) return p;
         if (level > 0) continue;
         // the longest rows: one tile of which the LDS holds eight rows
@@ -308,7 +309,7 @@ static Mx4Shape mx4_shape(int type, int dim, int level, bool wide) {
         p.r = 8;
         p.u = 8;
         p.ksu = (ks + 7) / 8 * 8;
-        p.lds = (size_t)p.ksu * 2048 + one.qpt * sizeof(float);
+        p.lds = (size_t)p.ksu * 2048 + (size_t)one.qpt * 8;
         p.qb = one.qpt / 2;
         return p;
     }

@@ -76,15 +76,22 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
     return v;
 }
-// 1 / |x| of one row by one wave: the sum of squares in fp64, rounded once (a zero row keeps its zeros)
-__device__ __forceinline__ float wave_inv_norm(const void* row, int type, int dim, int lane) {
+// 1 / |x| of one row by one wave, as a power of two and a factor: |2^k x| lies in [1/2, 1) whatever the norm, and the factor, in (1, 2],
+// is rounded once.  The sum of squares is one of fp64; a zero row keeps its zeros, one that is not finite becomes NaN.
+__device__ __forceinline__ float wave_inv_norm(const void* row, int type, int dim, int lane, int& k) {
     double ss = 0.0;
     for (int i = lane; i < dim; i += 64) {
         const double x = (double)mx4_elem(row, type, i);
         ss = fma(x, x, ss);
     }
     ss = wave_sum_f64(ss);
-    return ss > 0.0 ? (float)fmin(1.0 / sqrt(ss), (double)FLT_MAX) : ss == 0.0 ? 1.f : (float)ss;      // NaN stays NaN
+    k = 0;
+    if (ss == 0.0) return 1.f;
+    if (!(ss <= DBL_MAX)) return NAN;
+    int e;
+    const double m = frexp(sqrt(ss), &e);
+    k = -e;
+    return (float)(1.0 / m);
 }
 
 }  // namespace rag

@@ -93,9 +93,10 @@ __device__ __forceinline__ unsigned mx4_head2(float x, float y) { return __built
 template <int P>
 struct Mx4Split {
     int w[P][4];
-    // elements 2 j and 2 j + 1
-    __device__ __forceinline__ void pair(const Mx4Raw<P>& raw, int j) {
-        if constexpr (P == 1) {                                  // as they are; an infinity becomes a NaN
+    // elements 2 j and 2 j + 1; SCALED: times 2^k, exactly
+    template <bool SCALED>
+    __device__ __forceinline__ void pair(const Mx4Raw<P>& raw, int j, int k) {
+        if constexpr (P == 1 && !SCALED) {                       // as they are; an infinity becomes a NaN
             const unsigned x = (unsigned)raw.w[j], lo = (x & 0x7f80u) == 0x7f80u ? 0x40u : 0u, hi = (x & 0x7f800000u) == 0x7f800000u ? 0x400000u : 0u;
             w[0][j] = (int)(x | lo | hi);
         } else {
@@ -103,9 +104,16 @@ struct Mx4Split {
             if constexpr (P == 3) {
                 x = __int_as_float(raw.w[2 * j]);
                 y = __int_as_float(raw.w[2 * j + 1]);
-            } else {
+            } else if constexpr (P == 2) {
                 x = f16_f32((unsigned short)(unsigned)raw.w[j]);              // (an infinity's second part is NaN)
                 y = f16_f32((unsigned short)((unsigned)raw.w[j] >> 16));
+            } else {
+                x = bf16_f32((unsigned)raw.w[j] & 0xffffu);
+                y = __uint_as_float((unsigned)raw.w[j] & 0xffff0000u);
+            }
+            if constexpr (SCALED) {
+                x = ldexpf(x, k);
+                y = ldexpf(y, k);
             }
 #pragma unroll
             for (int p = 0; p + 1 < P; ++p) {
@@ -117,9 +125,11 @@ struct Mx4Split {
             w[P - 1][j] = (int)(__float_as_uint(x) >> 16 | (__float_as_uint(y) & 0xffff0000u));
         }
     }
-    // Where an element would round beyond the range, or is beyond it, all of them again.  (Only fp32 elements can.)
+    // Where an element would round beyond the range, or is beyond it, all of them again.  (Only fp32 elements can; scaled ones do not,
+    // and a query that is not finite has a factor that makes its scores NaN.)
+    template <bool SCALED>
     __device__ __forceinline__ void finish(const Mx4Raw<P>& raw) {
-        if constexpr (P == 3) {
+        if constexpr (P == 3 && !SCALED) {
             unsigned most = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -156,15 +166,18 @@ struct Mx4Split {
     }
 };
 
-// COSINE: what the queries' scores are multiplied with at the end (else 1)
+// COSINE: the queries are multiplied with 2^k before they are split, so that neither their parts nor their sums leave the range, and
+// the scores with inv
 template <int P, int QB, int NT>
-__device__ __forceinline__ void mx4_query_norms(const Mx4ScoreArgs& a, const char* q, int nqh, float* inv) {
+__device__ __forceinline__ void mx4_query_norms(const Mx4ScoreArgs& a, const char* q, int nqh, float* inv, int* k) {
     constexpr int ESIZE = P == 3 ? 4 : 2, TYPE = P == 3 ? RAG_MX4_F32 : P == 2 ? RAG_MX4_F16 : RAG_MX4_BF16;
     if (a.normalize) {
         for (int s = threadIdx.x >> 6; s < nqh; s += NT / 64) {
-            const float f = wave_inv_norm(q + (size_t)s * a.ldq * ESIZE, TYPE, a.dim, threadIdx.x & 63);
-            if ((threadIdx.x & 63) == 0) inv[s] = f;
+            int e;
+            const float f = wave_inv_norm(q + (size_t)s * a.ldq * ESIZE, TYPE, a.dim, threadIdx.x & 63, e);
+            if ((threadIdx.x & 63) == 0) { inv[s] = f; k[s] = e; }
         }
+        __syncthreads();
     } else {
         for (int s = threadIdx.x; s < QB; s += NT) inv[s] = 1.f;
     }
@@ -173,11 +186,11 @@ __device__ __forceinline__ void mx4_query_norms(const Mx4ScoreArgs& a, const cha
 // queries [q0, q0 + nqh) -> their parts in LDS, block after block.  Blocks past the row's are zero: they meet a real block of the
 // row again.  What the fragments of absent queries hold does not matter: it stays in result rows that nobody reads.
 template <int P, int QPT, int MT, int R, int NT>
-__device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, const char* q, int nqh, uint8_t* frag, float* inv) {
+__device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, const char* q, int nqh, uint8_t* frag, float* inv, int* k) {
     typedef Mx4Tiles<P, QPT, MT> L;
     constexpr int ESIZE = P == 3 ? 4 : 2, BLOCK = MT * R * 256;
     const int tid = threadIdx.x;
-    mx4_query_norms<P, L::QB, NT>(a, q, nqh, inv);
+    mx4_query_norms<P, L::QB, NT>(a, q, nqh, inv, k);
     if (a.ksu > a.ks) {
         const v4i zero = {0, 0, 0, 0};
         v4i* f = reinterpret_cast<v4i*>(frag + a.ks * BLOCK);
@@ -185,8 +198,9 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, const c
     }
     // a few units at once, so that their fetches are under way together (behind the last unit: that one again)
     const int units = nqh * a.ks * 16;
-    auto stage = [&](auto together) {
+    auto stage = [&](auto together, auto scaled) {
         constexpr int N = decltype(together)::value;
+        constexpr bool SCALED = decltype(scaled)::value;
         for (int u0 = tid; u0 < units; u0 += NT * N) {
             Mx4Raw<P> raw[N];
             int s[N], unit[N];
@@ -202,14 +216,16 @@ __device__ __forceinline__ void mx4_stage_queries(const Mx4ScoreArgs& a, const c
                 if (j > 0 && u0 + j * NT >= units) break;
                 Mx4Split<P> parts;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) parts.pair(raw[j], i);
-                parts.finish(raw[j]);
+                for (int i = 0; i < 4; ++i) parts.template pair<SCALED>(raw[j], i, SCALED ? k[s[j]] : 0);
+                parts.template finish<SCALED>(raw[j]);
                 parts.template store<QPT, MT, R>(s[j], unit[j] & 15, frag + (unit[j] >> 4) * BLOCK);
             }
         }
     };
-    if (units <= NT) stage(std::integral_constant<int, 1>{});
-    else stage(std::integral_constant<int, 4>{});
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 4> Four;
+    if (a.normalize) units <= NT ? stage(One{}, std::true_type{}) : stage(Four{}, std::true_type{});
+    else units <= NT ? stage(One{}, std::false_type{}) : stage(Four{}, std::false_type{});
     __syncthreads();
 }
 
@@ -319,6 +335,7 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     uint8_t* frag = smem;
     float* inv = reinterpret_cast<float*>(frag + ksu * BLOCK);
+    int* kexp = reinterpret_cast<int*>(inv + L::QB);
 
     // this wave takes the tiles of 16 rows first, first + stride, ... (LONG: four from each)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -420,7 +437,7 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     Buf x, y;
     int t = first;
     load(x, t, 0);                                              // on its way while the queries are split
-    mx4_stage_queries<P, QPT, MT, R, NW * 64>(a, static_cast<const char*>(a.q) + (size_t)w.q0 * a.ldq * (P == 3 ? 4 : 2), nqh, frag, inv);
+    mx4_stage_queries<P, QPT, MT, R, NW * 64>(a, static_cast<const char*>(a.q) + (size_t)w.q0 * a.ldq * (P == 3 ? 4 : 2), nqh, frag, inv, kexp);
     if (first >= end) return;
 #pragma unroll
     for (int set = 0; set < L::SETS; ++set)
@@ -528,6 +545,7 @@ __global__ __launch_bounds__(512) void mx4_scores_many_kernel(Mx4ScoreArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     uint8_t* frag = smem;
     float* inv = reinterpret_cast<float*>(frag + (WHOLE ? a.ks : 2) * BLOCK);
+    int* kexp = reinterpret_cast<int*>(inv + QB);
     Mx4Work w;
     if (!mx4_work(a, QB, w)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -543,7 +561,7 @@ __global__ __launch_bounds__(512) void mx4_scores_many_kernel(Mx4ScoreArgs a) {
     };
     const int l0 = (int)(w.row0 & 15) + n16;                    // tiles start at multiples of 16 from row0
     const int wo = (l0 >> 4) * 16 * a.code_ld + (l0 & 15) * 64 + col * 16, so = n16 * a.scale_ld + col * 4;
-    auto load = [&](Buf& b, int tile, int k) {
+    auto load = [&](Buf& b, int tile, int k) __attribute__((always_inline)) {
         const Mx4Rows from(a, w.row0 + (long long)(tile < tiles ? tile : tiles - 1) * (16 * NB));
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -553,7 +571,7 @@ __global__ __launch_bounds__(512) void mx4_scores_many_kernel(Mx4ScoreArgs a) {
     };
     // the queries' units of block k: query u / 16 (an absent one: the last again), elements 8 (u % 16) of the block
     Mx4Raw<P> raw[UPT];
-    auto fetch_queries = [&](int k) {
+    auto fetch_queries = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < UPT; ++j) {
             const int u = tid + j * NT, s = u >> 4 < nqh ? u >> 4 : nqh - 1;
@@ -561,15 +579,16 @@ __global__ __launch_bounds__(512) void mx4_scores_many_kernel(Mx4ScoreArgs a) {
         }
     };
     Mx4Split<P> parts[UPT];
-    auto split_pair = [&](int i) {
+    int scale[UPT];                                             // COSINE
+    auto split_pair = [&](int i, auto scaled) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < UPT; ++j) parts[j].pair(raw[j], i);
+        for (int j = 0; j < UPT; ++j) parts[j].template pair<decltype(scaled)::value>(raw[j], i, scale[j]);
     };
-    auto put_queries = [&](uint8_t* to) {
+    auto put_queries = [&](uint8_t* to, auto scaled) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < UPT; ++j) {
             const int u = tid + j * NT;
-            parts[j].finish(raw[j]);
+            parts[j].template finish<decltype(scaled)::value>(raw[j]);
             if (UNITS % NT == 0 || u < UNITS) parts[j].template store<QPT, MT, R>(u >> 4, u & 15, to);
         }
     };
@@ -577,19 +596,19 @@ __global__ __launch_bounds__(512) void mx4_scores_many_kernel(Mx4ScoreArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) at[i] = mx4_frag_at<R>(i, col, n16);
     v4f acc[MT][NB];
-    auto clear = [&] {
+    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) acc[mt][nb] = (v4f){0.f, 0.f, 0.f, 0.f};
     };
-    auto multiply = [&](const Buf& b, int k, const uint8_t* f, auto meanwhile) {
+    auto multiply = [&](const Buf& b, int k, const uint8_t* f, auto meanwhile) __attribute__((always_inline)) {
         constexpr int AHEAD = 2, RING = AHEAD + 1, ALL = 4 * MT;
         v8bf x[RING], y[2][NB];
         float scale[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) scale[nb] = mx4_scale(b.s[nb], k & 3);
-        auto fetch = [&](auto ic) {
+        auto fetch = [&](auto ic) __attribute__((always_inline)) {
             constexpr int n = decltype(ic)::value, i = n / MT, mt = n % MT;
             x[n % RING] = *reinterpret_cast<const v8bf*>(f + mt * R * 256 + at[i]);
         };
@@ -610,7 +629,7 @@ __global__ __launch_bounds__(512) void mx4_scores_many_kernel(Mx4ScoreArgs a) {
             __builtin_amdgcn_sched_barrier(0);
         });
     };
-    auto store = [&](int tile) {
+    auto store = [&](int tile) __attribute__((always_inline)) {
         const int r = tile * (16 * NB), left = rows - r < 16 * NB ? (rows - r) * 4 : 64 * NB;
 #pragma unroll
         for (int set = 0; set < L::SETS; ++set)
@@ -633,7 +652,7 @@ __global__ __launch_bounds__(512) void mx4_scores_many_kernel(Mx4ScoreArgs a) {
     int t = wave, k = 0;
     load(x, t, 0);
     if constexpr (WHOLE) {
-        mx4_stage_queries<P, QPT, MT, R, NT>(a, q, nqh, frag, inv);
+        mx4_stage_queries<P, QPT, MT, R, NT>(a, q, nqh, frag, inv, kexp);
         if (t >= tiles) return;
         clear();
         auto turn = [&](const Buf& now, Buf& next) -> bool {
@@ -655,42 +674,51 @@ __global__ __launch_bounds__(512) void mx4_scores_many_kernel(Mx4ScoreArgs a) {
         }
     } else {
         // all waves of the workgroup take the same turns: those behind the last tile multiply it again and store nothing
-        int t0 = 0;
-        mx4_query_norms<P, QB, NT>(a, q, nqh, inv);
-        fetch_queries(0);
+        mx4_query_norms<P, QB, NT>(a, q, nqh, inv, kexp);
+        auto run = [&](auto scaled) __attribute__((always_inline)) {
+            int t0 = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_pair(i);
-        put_queries(frag);
-        fetch_queries(ks > 1 ? 1 : 0);
-        clear();
-        __syncthreads();
-        auto turn = [&](const Buf& now, Buf& next, const uint8_t* here, uint8_t* there) -> bool {
-            const int k2 = k + 1 < ks ? k + 1 : 0, t2 = k2 ? t : t + NW;
-            const bool last = !k2 && t0 + NW >= tiles;
-            load(next, t2, k2);
-            __builtin_amdgcn_sched_barrier(0);
-            // the next block's queries, fetched a turn ago, are split under the second half of the products
-            multiply(now, k, here, [&](auto ic) {
-                static_for<4>([&](auto pair) {
-                    if constexpr (decltype(ic)::value == 2 * MT + decltype(pair)::value * MT / 2) split_pair(decltype(pair)::value);
-                });
-            });
-            put_queries(there);
-            fetch_queries(k2 + 1 < ks ? k2 + 1 : 0);
-            if (!k2) {
-                if (t < tiles) store(t);
-                clear();
-                t0 += NW;
+            for (int j = 0; j < UPT; ++j) {
+                const int s = (tid + j * NT) >> 4;
+                scale[j] = decltype(scaled)::value ? kexp[s < nqh ? s : nqh - 1] : 0;
             }
-            t = t2;
-            k = k2;
+            fetch_queries(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) split_pair(i, scaled);
+            put_queries(frag, scaled);
+            fetch_queries(ks > 1 ? 1 : 0);
+            clear();
             __syncthreads();
-            return last;
+            auto turn = [&](const Buf& now, Buf& next, const uint8_t* here, uint8_t* there) __attribute__((always_inline)) -> bool {
+                const int k2 = k + 1 < ks ? k + 1 : 0, t2 = k2 ? t : t + NW;
+                const bool last = !k2 && t0 + NW >= tiles;
+                load(next, t2, k2);
+                __builtin_amdgcn_sched_barrier(0);
+                // the next block's queries, fetched a turn ago, are split under the second half of the products
+                multiply(now, k, here, [&](auto ic) {
+                    static_for<4>([&](auto pair) {
+                        if constexpr (decltype(ic)::value == 2 * MT + decltype(pair)::value * MT / 2) split_pair(decltype(pair)::value, scaled);
+                    });
+                });
+                put_queries(there, scaled);
+                fetch_queries(k2 + 1 < ks ? k2 + 1 : 0);
+                if (!k2) {
+                    if (t < tiles) store(t);
+                    clear();
+                    t0 += NW;
+                }
+                t = t2;
+                k = k2;
+                __syncthreads();
+                return last;
+            };
+            for (;;) {
+                if (turn(x, y, frag, frag + BLOCK)) break;
+                if (turn(y, x, frag + BLOCK, frag)) break;
+            }
         };
-        for (;;) {
-            if (turn(x, y, frag, frag + BLOCK)) break;
-            if (turn(y, x, frag + BLOCK, frag)) break;
-        }
+        if (a.normalize) run(std::true_type{});
+        else run(std::false_type{});
     }
 }
 

@@ -147,3 +147,64 @@ def test_queries_beyond_the_range_of_their_type_are_nan():
                     assert torch.isnan(got[1]).all()
                     got[1] = clean[1]
                     assert torch.equal(got, clean)
+
+
+def _unit(q64):
+    norm = np.linalg.norm(q64, axis=1, keepdims=True)
+    return q64 / np.where(norm > 0, norm, 1.0)              # (zero vectors stay zero)
+
+
+def _cosine_bound(unit64, v):
+    """product_bound of the unit queries; the factor that makes them so is rounded once (2^-24), its product with the sum again."""
+    return mx4.product_bound(unit64, v) + np.abs(mx4.scores(unit64, v)) * 2.0 ** -23 + 1e-37
+
+
+NORMS = [1e-43, 1e-40, 1e-38, 1e-36, 1e-33, 1e-28, 1e-20, 1.0, 1e5, 1e20, 1e30, 1e37, 1.2e38]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,n", [(33, 700), (768, 40_000), (1100, 30_000), (8192, 500)])
+def test_cosine_scores_of_queries_of_any_norm(dim, n, dtype):
+    """Few and many queries, whose elements are of the type's smallest to its largest size."""
+    import torch
+    rng = np.random.default_rng(dim + 20)
+    codes, scales = mx4.quantise(rng.standard_normal((256, dim)) / np.sqrt(dim))
+    v = mx4.values(codes, scales, dim)
+    at = rng.integers(0, 256, n)
+    from rag_amd import QuantizedIndex
+    index = QuantizedIndex.from_packed(codes[at], scales[at], dim, metric="cosine")
+    info = torch.finfo(_t(dtype))
+    for nq in (len(NORMS), 7 * len(NORMS)):
+        q = rng.uniform(-1, 1, (nq, dim)) * np.tile(NORMS, nq // len(NORMS))[:, None]
+        if dtype == "float16":
+            q = q / np.abs(q).max(1, keepdims=True) * np.exp2(rng.uniform(-23, 15.9, (nq, 1)))
+        q = torch.from_numpy(q.clip(-info.max, info.max).astype(np.float32)).to(_t(dtype)).cuda()
+        q64 = q.double().cpu().numpy()
+        unit = _unit(q64)
+        got = index.scores(q).cpu().numpy()
+        assert (np.abs(got - mx4.scores(unit, v)[:, at]) <= _cosine_bound(unit, v)[:, at]).all()
+        one = index.scores(q[:1]).cpu().numpy()
+        assert np.array_equal(one[0], got[0])
+    D, I = index.search(q[:len(NORMS)], 3)
+    assert np.array_equal(D.cpu().numpy(), np.sort(got[:len(NORMS)], 1)[:, ::-1][:, :3])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_grouped_cosine_scores(dtype):
+    """Pieces that begin behind the first query, of queries of very different norms."""
+    import torch
+    rng = np.random.default_rng(21)
+    small, index, at, v = _spread(rng, 384, 20_000)
+    index = type(index).from_packed(*index.packed(), 384, metric="cosine")
+    q = torch.from_numpy((rng.standard_normal((150, 384)) * np.exp2(rng.integers(-12, 12, (150, 1)))).astype(np.float32)).to(_t(dtype)).cuda()
+    q64 = q.double().cpu().numpy()
+    unit = _unit(q64)
+    want, bound = mx4.scores(unit, v), _cosine_bound(unit, v)
+    at = at.cpu().numpy()
+    for most in (1, 5, 40):
+        a, b = rng.integers(0, 140, 150), rng.integers(0, 19_000, 150)
+        groups = np.stack([a, np.minimum(150, a + rng.integers(0, most + 1, 150)), b, np.minimum(20_000, b + rng.integers(0, 1500, 150))], 1)
+        plan = index.plan_groups(groups, 150, q.dtype)
+        for got, (q0, q1, r0, r1) in zip(plan.split(index.scores_grouped(q, plan)), groups):
+            i = np.ix_(np.arange(q0, q1), at[r0:r1])
+            assert (np.abs(got.cpu().numpy() - want[i]) <= bound[i]).all()
