@@ -7,10 +7,12 @@ EVEN_FIRST = np.array([0, 2, 4, 6, 1, 3, 5, 7])
 
 
 def normalise(x32):
-    """Rows divided by their norm as the index does it: the factor rounded to float32, the products in float32."""
-    ss = (x32.astype(np.float64) ** 2).sum(1)
-    inv = np.where(ss > 0, 1.0 / np.sqrt(np.where(ss > 0, ss, 1.0)), 1.0).astype(np.float32)
-    return x32 * inv[:, None]
+    """Rows divided by their norm as the index does it: times the power of two that brings the norm into [1/2, 1), which is exact, then
+    times the rest of the factor, rounded to float32, in float32."""
+    norm = np.sqrt((x32.astype(np.float64) ** 2).sum(1))
+    m, e = np.frexp(np.where(norm > 0, norm, 0.5))
+    inv = np.where(norm > 0, 1.0 / m, 1.0).astype(np.float32)
+    return np.ldexp(x32, -e[:, None]) * inv[:, None]
 
 
 def quantise(x):

@@ -69,6 +69,7 @@ template <int TYPE, bool VEC, bool AT>
 __global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
     __shared__ long long s_to[MX4_ROWS];
     __shared__ float s_inv[MX4_ROWS];
+    __shared__ int s_exp[MX4_ROWS];
     __shared__ int s_late[MX4_ROWS];
     const long long i0 = (a.block0 + blockIdx.x) * a.per_block;
     const int nr = (int)(a.count - i0 < a.per_block ? a.count - i0 : a.per_block);
@@ -87,6 +88,7 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
         }
         s_to[tid] = to;
         s_inv[tid] = 1.f;
+        s_exp[tid] = 0;
         s_late[tid] = 0;
     }
     __syncthreads();
@@ -102,7 +104,7 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
         for (int r = tid >> 6; r < nr; r += 4) {
             int k;
             const float inv = wave_inv_norm(x + (size_t)r * a.ldx * ESIZE, TYPE, a.dim, lane, k);
-            if (lane == 0) s_inv[r] = inv == inv ? fminf(ldexpf(inv, k), FLT_MAX) : inv;
+            if (lane == 0) { s_inv[r] = inv; s_exp[r] = k; }
         }
         __syncthreads();
     }
@@ -123,10 +125,11 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
             const long long to = s_to[r];
             if (AT && to < 0) continue;                                // uniform over the four lanes of a group
             const float inv = s_inv[r];
+            const int k = s_exp[r];
             unsigned most = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                v[j][i] *= inv;
+                v[j][i] = ldexpf(v[j][i], k) * inv;              // (the power of two first, exactly: no norm leaves the range)
                 const unsigned m = __float_as_uint(v[j][i]) & 0x7fffffffu;
                 most = m > most ? m : most;
             }

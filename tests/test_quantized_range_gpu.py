@@ -208,3 +208,32 @@ def test_grouped_cosine_scores(dtype):
         for got, (q0, q1, r0, r1) in zip(plan.split(index.scores_grouped(q, plan)), groups):
             i = np.ix_(np.arange(q0, q1), at[r0:r1])
             assert (np.abs(got.cpu().numpy() - want[i]) <= bound[i]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [40, 768])
+def test_cosine_rows_of_any_norm_are_stored_as_unit_rows(dim, dtype):
+    """Appended, and written to named positions; a zero row stays zero."""
+    import torch
+    from rag_amd import QuantizedIndex
+    rng = np.random.default_rng(dim + 30)
+    info = torch.finfo(_t(dtype))
+    x = rng.uniform(-1, 1, (len(NORMS) * 5, dim)) * np.repeat(NORMS, 5)[:, None]
+    if dtype == "float16":
+        x = x / np.abs(x).max(1, keepdims=True) * np.exp2(rng.uniform(-23, 15.9, (len(x), 1)))
+    x[11] = 0
+    x = torch.from_numpy(x.clip(-info.max, info.max).astype(np.float32)).to(_t(dtype))
+    want = mx4.quantise(mx4.normalise(x.float().numpy()))
+    index = QuantizedIndex(dim)
+    index.add(x.cuda())
+    for again in range(2):
+        codes, scales = index.packed()
+        # a factor on a rounding border could differ in its last bit: at most one of the rows may
+        differ = (codes.cpu().numpy() != want[0]).any(1) | (scales.cpu().numpy() != want[1]).any(1)
+        assert differ.sum() <= 1 and not differ[11]
+        norm = np.linalg.norm(index.reconstruct(np.arange(len(x))), axis=1)
+        there = (x.float() != 0).any(1).numpy()
+        # a value is off by at most a third of itself or a quarter of its group's unit u, whose largest element is 3.5 u at least: the
+        # error's norm is at most sqrt(1 / 9 + 32 / 16 / 3.5^2) = 0.53 of the row's
+        assert (np.abs(norm[there] - 1) <= 0.53).all() and (norm[~there] == 0).all()
+        index.write(torch.arange(len(x), device="cuda").flip(0), x.cuda().flip(0))
