@@ -145,7 +145,8 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(Mx4WriteArgs a) {
             w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[j][4], v[j][5], scale, 2);
             w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[j][6], v[j][7], scale, 3);
             *reinterpret_cast<unsigned*>(a.codes + mx4_code_at(to, a.code_ld, c >> 4) + (c & 15) * 4) = bad ? 0u : w;
-            if ((c & 3) == 0) a.scales[(size_t)to * a.scale_ld + mx4_scale_at(c >> 2)] = bad ? 255 : (uint8_t)(e + 127);
+            if ((c & 3) == 0)                                            // (groups behind the row's end: zero)
+                a.scales[(size_t)to * a.scale_ld + mx4_scale_at(c >> 2)] = c * 8 >= a.dim ? 0 : bad ? 255 : (uint8_t)(e + 127);
         }
     }
 }

@@ -237,3 +237,18 @@ def test_cosine_rows_of_any_norm_are_stored_as_unit_rows(dim, dtype):
         # error's norm is at most sqrt(1 / 9 + 32 / 16 / 3.5^2) = 0.53 of the row's
         assert (np.abs(norm[there] - 1) <= 0.53).all() and (norm[~there] == 0).all()
         index.write(torch.arange(len(x), device="cuda").flip(0), x.cuda().flip(0))
+
+
+@pytest.mark.parametrize("dim", [1, 32, 33, 100, 128, 200, 520, 768])
+def test_written_rows_are_those_that_were_packed_byte_for_byte(dim):
+    """The store's own buffers: zeros behind a row's elements and groups however it came there."""
+    import torch
+    from rag_amd import QuantizedIndex
+    rng = np.random.default_rng(dim)
+    x = rng.standard_normal((50, dim)).astype(np.float32)
+    packed = QuantizedIndex.from_packed(*mx4.quantise(x), dim)
+    added = QuantizedIndex(dim, metric="ip", capacity=50)
+    added.add(torch.from_numpy(x).cuda())
+    for again in range(2):
+        assert torch.equal(added._codes, packed._codes) and torch.equal(added._scales, packed._scales)
+        added.write(np.arange(50), x)
