@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import logging
 import time
-from typing import Any, Dict, List, Optional, Sequence, Tuple
+from typing import Any, Dict, List, Mapping, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -28,7 +28,7 @@ _METRIC = {MetricType.COSINE: "cosine", MetricType.DOT_PRODUCT: "ip", MetricType
 
 
 def _four_bit(config: SearchConfig) -> bool:
-    return config.quantization_config is not None and "mx4" in config.quantization_config
+    return isinstance(config.quantization_config, Mapping) and "mx4" in config.quantization_config
 
 
 class HipSearchOptimizer:

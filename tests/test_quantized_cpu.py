@@ -166,3 +166,13 @@ def test_quantised_index_needs_a_gpu():
     from rag_amd import QuantizedIndex, RagHipError
     with pytest.raises(RagHipError):
         QuantizedIndex(16)
+
+
+def test_only_a_mapping_with_the_key_asks_for_four_bit_rows():
+    """Any other quantization_config that is given keeps its meaning (a compressed copy that is searched first)."""
+    from types import SimpleNamespace
+    from rag_amd.schemas import SearchConfig
+    from rag_amd.search_optimizer import _four_bit
+    for given, want in (({"mx4": {}}, True), ({"mx4": None}, True), ({"scalar": {"type": "int8"}}, False), ({}, False), (None, False), (True, False),
+                        (SimpleNamespace(scalar=1), False), ("mx4", False), (object(), False)):
+        assert _four_bit(SearchConfig(dimension=8, quantization_config=given)) is want, given
