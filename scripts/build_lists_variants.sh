@@ -7,7 +7,7 @@ mkdir -p build/variants
 while [ $# -ge 2 ]; do
   name=$1; flags=$2; shift 2
   (
-    /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=off $flags -c rag_amd/csrc/ivf_lists.hip -o build/variants/lists_$name.o
+    /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops $flags -c rag_amd/csrc/ivf_lists.hip -o build/variants/lists_$name.o
     objs=$(ls rag_amd/csrc/*.o | grep -v ivf_lists.o)
     /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC $objs build/variants/lists_$name.o -o build/variants/librag_hip_$name.so
     echo built $name
