@@ -252,3 +252,24 @@ def test_written_rows_are_those_that_were_packed_byte_for_byte(dim):
     for again in range(2):
         assert torch.equal(added._codes, packed._codes) and torch.equal(added._scales, packed._scales)
         added.write(np.arange(50), x)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,n", [(96, 50), (768, 1003), (768, 40_013), (1300, 30_001), (8192, 300)])
+def test_what_lies_around_the_scores_is_left_as_it_was(dim, n, dtype):
+    """Through the C entry point: rows of results that lie apart, before and behind them other data."""
+    import ctypes as C
+    import torch
+    from rag_amd import _lib
+    rng = np.random.default_rng(n)
+    _, index, _, _ = _spread(rng, dim, n)
+    for nq in (1, 5, 9, 40, 131):
+        q = torch.from_numpy(rng.standard_normal((nq, dim)).astype(np.float32)).to(_t(dtype)).cuda()
+        for begin, end in ((0, n), (7, n - 3)):
+            want = index.scores(q, begin, end)
+            room = torch.full((nq + 2, end - begin + 37), 7.0, device="cuda")
+            _lib.check(_lib.lib.rag_mx4_scores_device(C.byref(index._st), begin, end, nq, q.data_ptr(), TYPES.index(dtype), dim, 0, room[1:].data_ptr(),
+                                                      room.shape[1], torch.cuda.current_stream().cuda_stream))
+            assert torch.equal(room[1:-1, :end - begin], want)
+            room[1:-1, :end - begin] = 7.0
+            assert (room == 7.0).all()
