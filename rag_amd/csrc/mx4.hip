@@ -246,11 +246,12 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(Mx4ReadArgs a) {
 
 // ------------------------------------------------------------------------------------------------ products (kernels: mx4_scores.h)
 constexpr long long MX4_MOST_ROWS = 8192;               // of a piece of a ragged group
-constexpr long long MX4_WIDE = 40 * 1000 * 1000;         // 12 * 4 bytes * this, and a tile, stay below 2^31
+constexpr long long MX4_WIDE = 100 * 1000 * 1000;        // 3 * 4 bytes * this, and a tile, stay below 2^31
+constexpr long long MX4_BEYOND = 1LL << 37;              // scores, more than the memory of a card holds
 
 // The shapes of a type, by the queries of a workgroup: those of the kernel for few queries, then those of the one for many.  32 of
-// a type's queries and more go to the latter, whose fragments serve several row blocks; fp32 queries from 9 on, three of whose tiles would
-// take as many LDS reads as there are there (16 x 4M x 768: 405 us)
+// a type's queries and more go to the latter, whose fragments serve several row blocks; fp32 queries from 9 on, since the fragments of
+// their three tiles, read for every block of rows, would take all that the LDS gives at the rate of HBM (16 x 4M x 768: 405 us)
 struct Mx4Level {
     int qpt, mt, nb;             // nb 0: the kernel for few queries
 };
@@ -274,9 +275,10 @@ static int mx4_level_for(int type, long long nq) {
     while (level + 1 < mx4_levels(type).count && mx4_most(type, level) < nq) ++level;
     return level;
 }
-// The shape of a level, or of the next lower one that there is for rows of this length.  wide: the scores of two queries may lie
-// further apart than a lane's 32-bit offset reaches (the kernel for up to 8 queries of a large store has a base for each)
-static Mx4Shape mx4_shape(int type, int dim, int level, bool wide) {
+// The shape of a level, or of the next lower one that there is for rows of this length.  apart: how far apart the scores of two queries may
+// lie.  Beyond a lane's 32-bit offset each query needs a base of its own: the kernel for many has them, and that for up to 8 of a large
+// store.  (A plan for more scores than there can be keeps the pieces of 8 queries.)
+static Mx4Shape mx4_shape(int type, int dim, int level, long long apart) {
     constexpr int LDS = 160 * 1024;
     const int ks = mx4_blocks(dim);
     Mx4Shape p = {};
@@ -288,7 +290,7 @@ static Mx4Shape mx4_shape(int type, int dim, int level, bool wide) {
         p.qb = mx4_most(type, level);
         p.many = v.nb > 0;
         p.r = 16;
-        if (wide && (p.many || p.qb > 8)) continue;
+        if (apart > MX4_BEYOND ? p.qb > 8 : apart > MX4_WIDE && !p.many && p.qb > 8) continue;
         if (p.many) {
             p.nw = 8;
             p.ksu = ks;
@@ -298,7 +300,7 @@ static Mx4Shape mx4_shape(int type, int dim, int level, bool wide) {
             if (!p.steps) p.lds = (size_t)2 * p.mt * 4096 + factors;
             return p;
         }
-        p.big = wide;
+        p.big = apart > MX4_WIDE;
         p.nb = 1;
         p.steps = ks <= 8 && ks != 5 && ks != 7;
         p.u = p.steps ? ks : (ks & 7) == 0 || (ks & 7) > 4 ? 8 : 4;      // (blocks past the row's are fetched again, from the caches)
@@ -322,10 +324,10 @@ static Mx4Shape mx4_shape(int type, int dim, int level, bool wide) {
 // leave more than half of the compute units idle (32 fp32 queries x 10k x 768: 7.8 us, asked to fill a quarter of them 9.3; x 40k 14.6, 17.0;
 // 64 bf16 queries x 2000 x 1024: 5.6, 7.8)
 template <typename Units>
-static Mx4Shape mx4_shape_for(int type, int dim, long long nq, bool wide, Units groups_of) {
+static Mx4Shape mx4_shape_for(int type, int dim, long long nq, long long apart, Units groups_of) {
     int level = mx4_level_for(type, nq);
-    Mx4Shape p = mx4_shape(type, dim, level, wide);
-    while (level > 0 && groups_of(p) < 128) p = mx4_shape(type, dim, --level, wide);
+    Mx4Shape p = mx4_shape(type, dim, level, apart);
+    while (level > 0 && groups_of(p) < 128) p = mx4_shape(type, dim, --level, apart);
     return p;
 }
 
@@ -380,12 +382,13 @@ static Mx4ScoreArgs mx4_score_args(const rag_mx4_store_t* st, const Mx4Shape& p,
 // scores of rows [row0, row0 + rows) (checked by the caller)
 static int mx4_scores(const rag_mx4_store_t* st, long long row0, long long rows, long long nq, const void* q, int q_type, long long ldq,
                       int normalize, float* out, long long out_ld, hipStream_t s) {
-    Mx4Shape p = mx4_shape_for(q_type, st->dim, nq, out_ld > MX4_WIDE, [&](const Mx4Shape& s) {
+    Mx4Shape p = mx4_shape_for(q_type, st->dim, nq, out_ld, [&](const Mx4Shape& s) {
         return (rows + 16LL * s.nb * s.nw - 1) / (16LL * s.nb * s.nw) * ((nq + s.qb - 1) / s.qb);
     });
     Mx4ScoreArgs a = mx4_score_args(st, p, q, ldq, normalize, out);
-    // Past the caches once the rows exceed the 256 MB that they keep from call to call, and for up to 8 queries, whose waves then
-    // take 64 rows at a time, once these keep the waves busy
+    // Past the caches once the rows exceed the 256 MB that they keep from call to call (one query x 600k x 768, 250 MB: 39 us kept, 46 past
+    // them; 800k 61.6 and 59.3; 16 bf16 queries x 800k 80 and 73), and for up to 8 queries, whose waves then take 64 rows at a
+    // time, once these keep the waves busy (130k x 4096: 52 us in pieces of 64 rows, 48 of 16)
     p.big = p.big || (!p.many && nq <= p.qb && rows * (a.code_ld + a.scale_ld) > 256LL << 20 && (p.qb > 8 || rows >= 64 * 4096));
     a.row0 = row0;
     a.rows = rows;
@@ -665,7 +668,8 @@ int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngro
     *total = sum;
     // rows of a piece: enough pieces to fill the chip several times over, each long enough to pay for staging its queries;
     // with one tile, where that costs little and more workgroups fit a compute unit, shorter ones (1000 groups of 3 fp32
-    // queries x 2000 rows x 384: 106 us in pieces of 2048, 90 of 512)
+    // queries x 2000 rows x 384: 96.7 us in pieces of 1024, 92.6 of 512); with many queries four units of rows at least (100 groups of 40
+    // bf16 queries x 4000 x 768: 57 us, in pieces of three, two and one 71, 63 and 78)
     long long part = 0;
     auto queries = [&](long long g) { return (uint32_t)(groups[4 * g + 1] - groups[4 * g]); };
     auto rows = [&](long long g) { return (uint32_t)(groups[4 * g + 3] - groups[4 * g + 2]); };
@@ -680,14 +684,14 @@ int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngro
             items += (long long)parts(queries(g), s.qb) * parts(rows(g), (uint32_t)part);
         return items;
     };
-    const Mx4Shape p = mx4_shape_for(q_type, dim, std::max<long long>(most_q, 1), sum > MX4_WIDE, cut);       // (no group has more rows than scores)
+    const Mx4Shape p = mx4_shape_for(q_type, dim, std::max<long long>(most_q, 1), sum, cut);       // (no group has more rows than scores)
     const long long pieces = cut(p);
     if (pieces > 0x7fffffffLL) return fail(RAG_ERR_INVALID, "too many pieces");
     *widest = (int32_t)std::min<long long>(most_q, p.qb);
     *n_items = pieces;
     if (pieces > max_items) return RAG_OK;
     // The longest pieces first, so that the last workgroups to begin are the short ones (200 groups of up to 24 fp16 queries x
-    // 3000 rows x 384: 32.4 us in the groups' order, 28.5 like this; 512 lists of 400 rows x 1024: 24.2, 22.0)
+    // 3000 rows x 384: 50.3 us in the groups' order, 41.6 like this; 512 lists of 400 rows x 1024: 24.3, 23.8)
     constexpr int CLASSES = MX4_MOST_ROWS / 16;
     int64_t place[CLASSES] = {};                          // pieces of each (rows - 1) / 16, then where the next one of them goes
     for (long long g = 0; g < ngroups; ++g) {
@@ -763,7 +767,7 @@ int rag_mx4_scores_grouped_device(const rag_mx4_store_t* st, int64_t nq, const v
     if (widest < 1 || widest > nq) return fail(RAG_ERR_INVALID, "widest is not what rag_mx4_plan_groups gave for these queries");
     Mx4DeviceGuard g(st->device);
     if (!g.ok) return fail(RAG_ERR_HIP, "hipSetDevice failed");
-    const Mx4Shape p = mx4_shape(q_type, st->dim, mx4_level_for(q_type, widest), total > MX4_WIDE);
+    const Mx4Shape p = mx4_shape(q_type, st->dim, mx4_level_for(q_type, widest), total);
     Mx4ScoreArgs a = mx4_score_args(st, p, q_dev, q_stride, normalize ? 1 : 0, out_dev);
     a.nq = (int)nq;
     a.rows = st->n;

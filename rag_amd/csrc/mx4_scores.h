@@ -22,23 +22,25 @@ namespace rag {
 // 8 i .. 8 i + 7 of every lane's group.
 //
 // QPT: queries of a tile of 16 rows of parts.  16 / QPT rows each (4: the three parts of an fp32 query, or those of fewer queries
-// than a tile holds); 16 for fp32 (SPLIT): three tiles hold the three parts of sixteen queries.
+// than a tile holds); 16 for fp32 (SPLIT): three tiles hold the three parts of sixteen queries.  Queries go to the columns of lanes
+// in turn, so that the scores of a store lie at most three queries apart, which a lane's 32-bit offset has to reach.
 template <int P, int QPT, int MT>
 struct Mx4Tiles {
     static constexpr bool SPLIT = P == 3 && QPT == 16;
     static constexpr int ROWS = 16 / QPT;                        // rows of a tile per query
     static constexpr int SETS = SPLIT ? MT / 3 : MT;             // sets of tiles with QPT queries each
-    static constexpr int SPL = QPT / 4;                          // queries of a set whose scores a lane holds: c * SPL + j
+    static constexpr int SPL = QPT / 4;                          // queries of a set whose scores a lane of column c holds: 4 j + c
     static constexpr int QB = SETS * QPT;
     static_assert(SPLIT ? MT % 3 == 0 : ROWS >= P, "");
 };
 
-// Where part p of query s of a set begins: (tile, row)
-template <int P, int QPT, int MT>
+// Where part p of query s lies: (tile, row).  Of a tile of R = 8 rows two columns hold queries.
+template <int P, int QPT, int MT, int R>
 __device__ __forceinline__ void mx4_part_at(int s, int p, int& tile, int& m) {
     typedef Mx4Tiles<P, QPT, MT> L;
+    constexpr int COLS = R / 4;
     tile = L::SPLIT ? s / 16 * 3 + p : s / QPT;
-    m = L::SPLIT ? s % 16 : s % QPT * L::ROWS + p;
+    m = s % COLS * 4 + s % QPT / COLS * L::ROWS + (L::SPLIT ? 0 : p);
 }
 
 // A block of a tile in LDS: four steps of R rows x 4 columns x 16 bytes.  A lane's place among its column's is its row number
@@ -160,7 +162,7 @@ struct Mx4Split {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             int tile, m;
-            mx4_part_at<P, QPT, MT>(s, p, tile, m);
+            mx4_part_at<P, QPT, MT, R>(s, p, tile, m);
             *reinterpret_cast<v4i*>(frag + tile * R * 256 + mx4_frag_at<R>(unit & 3, (unit >> 2) & 3, m)) = (v4i){w[p][0], w[p][1], w[p][2], w[p][3]};
         }
     }
@@ -329,7 +331,7 @@ constexpr unsigned MX4_NOWHERE = 0x80000000u;                    // an offset be
 template <int P, int QPT, int MT, int R, int U, int NW, int STEPS, bool BIG>
 __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     typedef Mx4Tiles<P, QPT, MT> L;
-    constexpr int QB = L::QB * R / 16, BLOCK = MT * R * 256;
+    constexpr int QB = L::QB * R / 16, BLOCK = MT * R * 256, COLS = R / 4;
     constexpr bool LONG = BIG && QB <= 8;
     const int ks = STEPS ? U : a.ks, ksu = STEPS ? U : a.ksu;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -424,12 +426,12 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
                     const int r = (tile - 3) * 16, left = rows - r < 64 ? (rows - r) * 4 : 256;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const int query = set * QPT + c * L::SPL + j;
-                        if (query < QB) mx4_put(held[set][j][c], out + query * ld + r, query < nqh ? left : 0, lane * 4);
+                        const int query = set * QPT + j * COLS + c;
+                        if (c < COLS) mx4_put(held[set][j][c], out + query * ld + r, query < nqh ? left : 0, lane * 4);
                     }
                 } else {
                     const int r = tile * 16;
-                    mx4_put(total(set, j), out + (set * QPT + j) * ld + r, 0x7fffffff, r + n16 < rows ? place[set][j] : MX4_NOWHERE);
+                    mx4_put(total(set, j), out + (set * QPT + j * COLS) * ld + r, 0x7fffffff, r + n16 < rows ? place[set][j] : MX4_NOWHERE);
                 }
             }
     };
@@ -443,9 +445,9 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
     for (int set = 0; set < L::SETS; ++set)
 #pragma unroll
         for (int j = 0; j < L::SPL; ++j) {
-            const int query = set * QPT + col * L::SPL + j;
+            const int query = set * QPT + j * COLS + col % COLS;
             iv[set][j] = inv[query];
-            place[set][j] = query < nqh ? (unsigned)(col * L::SPL * ld + n16) * 4u : MX4_NOWHERE;
+            place[set][j] = col < COLS && query < nqh ? (unsigned)(col * ld + n16) * 4u : MX4_NOWHERE;
         }
     auto hold = [&](auto sub) {
 #pragma unroll
@@ -532,10 +534,13 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
 // earlier: rows of any length take the same LDS, and one barrier a block stands against 4 MT NB products of every wave (256 fp32
 // queries x 200k x 768: 181 us, 207 like this; fetched in the block before only: 241).
 //
-// What bounds it: the matrix unit.  256 fp32 queries x 200k x 768 are 2.4e14 operations on the three parts, 1.3e15 a second, what a
-// large library product of bf16 matrices reaches on this card (the instruction alone: 2.0e15).  Four blocks per fragment instead of
-// three for 32 fp32 queries: the same time (184), and registers spill where the parts are made on the way.  bf16 queries have a third
-// of the products and are bound by these and the stores alike (111 us; 205 MB of scores are 42).
+// What bounds it, 256 fp32 queries x 200k x 768 (2.4e14 operations on the three parts): 186 to 189 us, 1.3e15 operations a second; a large
+// library product of bf16 matrices reaches as many on this card, the instruction alone 2.0e15.  With the products alone 131 us; all but the
+// products 146; all but the stores 158, all but the fetch of rows 164, all but the fragments' LDS reads 179, all but the unpacking 185.  So the
+// matrix unit (busy 55 % of the cycles), and stores and fetches that are not wholly hidden behind it: they share a counter, and behind the
+// branch that asks whether a row is done the compiler waits for the stores.  Rows fetched two blocks ahead, fragments three to six
+// ahead, and four row blocks to a fragment (184; where the parts are made on the way its registers spill) change nothing.  bf16 queries have a
+// third of the products: 107 to 112 us, of which 205 MB of scores are 42.
 template <int P, int QPT, int MT, int NB, bool WHOLE>
 __global__ __launch_bounds__(512) void mx4_scores_many_kernel(Mx4ScoreArgs a) {
     typedef Mx4Tiles<P, QPT, MT> L;
@@ -635,14 +640,14 @@ __global__ __launch_bounds__(512) void mx4_scores_many_kernel(Mx4ScoreArgs a) {
         for (int set = 0; set < L::SETS; ++set)
 #pragma unroll
             for (int j = 0; j < L::SPL; ++j) {
-                const float f = inv[set * QPT + col * L::SPL + j];
+                const float f = inv[set * QPT + j * 4 + col];
                 float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) v[nb] = mx4_sum<P, QPT, MT>(acc, set, nb, j) * f;
                 columns_transpose(v);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int query = set * QPT + c * L::SPL + j;
+                    const int query = set * QPT + j * 4 + c;
                     mx4_put(v[c], out + query * ld + r, query < nqh ? left : 0, lane * 4);
                 }
             }

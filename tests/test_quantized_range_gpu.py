@@ -273,3 +273,21 @@ def test_what_lies_around_the_scores_is_left_as_it_was(dim, n, dtype):
             assert torch.equal(room[1:-1, :end - begin], want)
             room[1:-1, :end - begin] = 7.0
             assert (room == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype,nq", [("float32", 16), ("float32", 20), ("float16", 20), ("bfloat16", 34), ("bfloat16", 20)])
+def test_large_batches_whose_results_lie_far_apart(dtype, nq):
+    """More than 2^31 bytes from query to query, for the kernels that take the most queries."""
+    import ctypes as C
+    import torch
+    from rag_amd import _lib
+    rng = np.random.default_rng(41)
+    n, stride = 70_000, 600_000_000
+    _, index, _, _ = _spread(rng, 96, n)
+    q = torch.from_numpy(rng.standard_normal((nq, 96)).astype(np.float32)).to(_t(dtype)).cuda()
+    want = index.scores(q)
+    out = torch.empty((nq - 1) * stride + n, dtype=torch.float32, device="cuda")
+    _lib.check(_lib.lib.rag_mx4_scores_device(C.byref(index._st), 0, n, nq, q.data_ptr(), TYPES.index(dtype), 96, 0, out.data_ptr(), stride,
+                                              torch.cuda.current_stream().cuda_stream))
+    for i in range(nq):
+        assert torch.equal(out[i * stride: i * stride + n], want[i]), i
