@@ -448,8 +448,8 @@ int rag_index_hybrid_mmr_batch_device(rag_index_t* h, int64_t nq, const float* q
  * kept within [-126, 125] (a = 0: -126); codes are the nearest table values to |x| / 2^s, ties to the even code, at most 6.
  * A group that holds a NaN or an infinity is stored as NaN.
  *
- * The buffers belong to the caller (rag_mx4_layout gives the bytes of a row); every call is enqueued on `stream` of
- * st->device and not synchronised, keeps nothing between calls and allocates nothing, so it may be captured into a graph.
+ * The buffers belong to the caller (rag_mx4_layout gives the bytes of a row); every call but rag_mx4_upload_groups is enqueued on
+ * `stream` of st->device and not synchronised, keeps nothing between calls and allocates nothing, so it may be captured into a graph.
  * Calls that write one store and calls that use it are ordered by the caller's streams. */
 enum rag_mx4_type { RAG_MX4_F32 = 0, RAG_MX4_BF16 = 1, RAG_MX4_F16 = 2 };
 typedef struct rag_mx4_store {
@@ -467,14 +467,18 @@ int rag_mx4_layout(int dim, int64_t* code_bytes, int64_t* scale_bytes);
  *   rows_dev NULL   to the rows [first, first + count)
  *   rows_dev        to the positions it names; a position outside [0, n) is skipped, of several rows for one position the last is
  *                   kept.  owner_dev: n int32, zero before the first such call; every call leaves them zero.
- *   normalize       1: every row is divided by its norm first (COSINE; sum of squares in fp64; a zero row stays zero) */
+ *   normalize       1: every row is divided by its norm first (COSINE; sum of squares in fp64; whatever the norm, subnormal elements
+ *                   too; a zero row stays zero) */
 int rag_mx4_write_device(const rag_mx4_store_t* st, int64_t first, const int64_t* rows_dev, int32_t* owner_dev, int64_t count,
                          const void* x_dev, int x_type, int64_t x_stride, int normalize, void* stream);
 /* out_dev[count][dim] (out_type, rounded once to nearest even) = the values of the rows at rows_dev; a position outside
  * [0, n) -- an unfilled slot of a search -- reads as zeros */
 int rag_mx4_read_device(const rag_mx4_store_t* st, const int64_t* rows_dev, int64_t count, void* out_dev, int out_type, void* stream);
-/* out_dev[i * out_stride + r - row_begin] = sum over the elements of q_i * value(row r), r in [row_begin, row_end): the product
- * itself, in fp32 (normalize 1: of q_i / |q_i|).  A query that holds a NaN or an infinity gets NaN against every row. */
+/* out_dev[i * out_stride + r - row_begin] = sum over the elements of q_i * value(row r), r in [row_begin, row_end).  Queries and rows
+ * enter the products as they are, whatever their exponents, subnormal elements too (a value beyond the range of fp32, which only scales
+ * from 253 on have, is an infinity); the products are summed in fp32, in an order that depends on the row's length alone, so a
+ * score is the same whatever it is computed together with.  normalize 1: of q_i / |q_i|, for any norm; a zero query scores
+ * zero.  A query that holds a NaN or an infinity gets NaN against every row. */
 int rag_mx4_scores_device(const rag_mx4_store_t* st, int64_t row_begin, int64_t row_end, int64_t nq, const void* q_dev, int q_type,
                           int64_t q_stride, int normalize, float* out_dev, int64_t out_stride, void* stream);
 /* The same for ragged groups: group g multiplies its queries [groups[4g], groups[4g + 1]) with its rows [groups[4g + 2],
@@ -484,7 +488,9 @@ int rag_mx4_scores_device(const rag_mx4_store_t* st, int64_t row_begin, int64_t 
  *   out_begin   NULL or, per group, where its scores start;  *total: how many there are;  *widest: most queries of
  *               a piece, for the product call
  * rag_mx4_upload_groups copies the pieces to device memory, enqueued on `stream` (refused while that is captured into a graph);
- * `items` may be changed once it returns.  There they serve any number of products with queries of this count and type over a store
+ * `items` may be changed once it returns.  Up to 4096 pieces go through page-locked blocks of 128 KiB, which the library allocates as
+ * they are needed, 64 at most, shares between threads and devices and keeps; of more pieces, or with every block on its way, the call
+ * waits for the stream.  There they serve any number of products with queries of this count and type over a store
  * of at least n rows; a piece that does not fit the store, the queries or the `total` scores of out_dev is left out. */
 #define RAG_MX4_ITEM_BYTES 32
 int rag_mx4_plan_groups(int dim, int q_type, int64_t nq, int64_t n, int64_t ngroups, const int64_t* groups, int64_t max_items,

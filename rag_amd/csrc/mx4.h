@@ -5,8 +5,8 @@
 
 namespace rag {
 
-// A row of `dim` elements is padded with zeros to ks = ceil(dim / 128) blocks of 128 (what one matrix instruction takes
-// along the row): 64 bytes, element 2j in the low half of byte j, 2j + 1 in the high half.  codes: sixteen rows lie together,
+// A row of `dim` elements is padded with zeros to ks = ceil(dim / 128) blocks of 128 (four steps of the
+// matrix instruction): 64 bytes, element 2j in the low half of byte j, 2j + 1 in the high half.  codes: sixteen rows lie together,
 // block by block -- [row / 16][block][row % 16][64 bytes] -- so that one load of a wave (a block of sixteen rows) is one
 // contiguous KiB: 4M rows of 768 against one query 292 us with the rows one behind the other, 264 us like this.
 // scales: row after row, one byte per group of 32; the bytes of four consecutive blocks lie together per group column, so that the lane
