@@ -475,10 +475,10 @@ int rag_mx4_write_device(const rag_mx4_store_t* st, int64_t first, const int64_t
  * [0, n) -- an unfilled slot of a search -- reads as zeros */
 int rag_mx4_read_device(const rag_mx4_store_t* st, const int64_t* rows_dev, int64_t count, void* out_dev, int out_type, void* stream);
 /* out_dev[i * out_stride + r - row_begin] = sum over the elements of q_i * value(row r), r in [row_begin, row_end).  Queries and rows
- * enter the products as they are, whatever their exponents, subnormal elements too (a value beyond the range of fp32, which only scales
- * from 253 on have, is an infinity); the products are summed in fp32, in an order that depends on the row's length alone, so a
- * score is the same whatever it is computed together with.  normalize 1: of q_i / |q_i|, for any norm; a zero query scores
- * zero.  A query that holds a NaN or an infinity gets NaN against every row. */
+ * enter the products as they are, whatever their exponents, subnormal elements too; the products are summed in fp32, in an order
+ * that depends on the row's length alone, so a score is the same whatever it is computed together with.  A row with a value beyond
+ * the range of fp32, which only packed scales of 253 and 254 give, has scores that are not finite.  normalize 1: of q_i / |q_i|, for
+ * any norm; a zero query scores zero.  A query that holds a NaN or an infinity gets NaN against every row. */
 int rag_mx4_scores_device(const rag_mx4_store_t* st, int64_t row_begin, int64_t row_end, int64_t nq, const void* q_dev, int q_type,
                           int64_t q_stride, int normalize, float* out_dev, int64_t out_stride, void* stream);
 /* The same for ragged groups: group g multiplies its queries [groups[4g], groups[4g + 1]) with its rows [groups[4g + 2],

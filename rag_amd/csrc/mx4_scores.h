@@ -1,5 +1,5 @@
-// Products of queries with four-bit rows.  Instantiated for fp32 queries in mx4_scores_f32.hip, for bf16 and fp16 ones in
-// mx4_scores_16.hip.
+// Products of queries with four-bit rows.  Instantiated for fp32, bf16 and fp16 queries in mx4_scores_f32.hip, _bf16.hip and
+// _f16.hip.
 //
 // A product is that of the numbers themselves: no bit of a query or a row is left out, only the sums are rounded.  A four-bit
 // value times its power of two is a bf16 number (the conversion makes it with one instruction for two of them, subnormal ones
@@ -374,8 +374,9 @@ __global__ __launch_bounds__(NW * 64) void mx4_scores_kernel(Mx4ScoreArgs a) {
         }
 #pragma unroll
         for (int d = 0; d < SW; ++d) {
-            const int k = (ks0 >> 2) + d < sd ? (ks0 >> 2) + d : sd - 1;
-            b.s[d] = (int)__builtin_amdgcn_raw_buffer_load_b32(from.scales, so, k * 16, 0);
+            // (scales behind the row's are zero, here or in memory: those blocks' values are finite, and nothing beside zeros)
+            const bool there = STEPS || (ks0 >> 2) + d < sd;
+            b.s[d] = (int)__builtin_amdgcn_raw_buffer_load_b32(from.scales, there ? so : (int)MX4_NOWHERE, there ? ((ks0 >> 2) + d) * 16 : 0, 0);
         }
     };
     v4f acc[MT][1];

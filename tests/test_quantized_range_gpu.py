@@ -291,3 +291,29 @@ def test_large_batches_whose_results_lie_far_apart(dtype, nq):
                                               torch.cuda.current_stream().cuda_stream))
     for i in range(nq):
         assert torch.equal(out[i * stride: i * stride + n], want[i]), i
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [33, 520, 640, 1200, 5200, 5300, 8000])
+def test_rows_with_values_beyond_the_range(dim, dtype):
+    """Packed rows whose scale takes a value out of fp32: their scores are not finite, in single queries and batches alike; those of the
+    rows around them are."""
+    import torch
+    from rag_amd import QuantizedIndex
+    g = (dim + 31) // 32
+    n = 3 * g
+    codes, scales = np.full((n, 16 * g), 0x22, np.uint8), np.full((n, g), 100, np.uint8)      # ones, times 2^-27
+    row = np.arange(n)
+    codes.reshape(n, g, 16)[row, row // 3] = np.array([0x66, 0xEE, 0x22])[row % 3][:, None]
+    scales[row, row // 3] = np.array([254, 254, 100])[row % 3]                                  # 4 times 2^127, its negative, or ones again
+    index = QuantizedIndex.from_packed(codes, scales, dim)
+    big = QuantizedIndex.from_packed(np.tile(codes, (1 + 40_000 // n, 1)), np.tile(scales, (1 + 40_000 // n, 1)), dim)
+    for nq in (1, 5, 20, 130):
+        q = torch.rand((nq, dim), device="cuda").add_(0.5).to(_t(dtype))
+        got = torch.cat([index.scores(q[i:i + 1]) for i in range(nq)])
+        assert torch.equal(torch.isfinite(got), torch.from_numpy(row % 3 == 2).cuda().expand(nq, n)), nq
+        if dtype == "bfloat16":
+            assert (got[:, 0::3] == np.inf).all() and (got[:, 1::3] == -np.inf).all()
+        for other in (index.scores(q), big.scores(q)):
+            want = got.repeat(1, other.shape[1] // n)
+            assert torch.equal(torch.isnan(other), torch.isnan(want)) and torch.equal(torch.nan_to_num(other), torch.nan_to_num(want)), nq
